@@ -31,12 +31,14 @@ class DType(enum.IntEnum):
     BF16 = 2
     FP8_E4M3 = 3
     INT8 = 4
+    INT4 = 5  # pools only
 
 
 class ScaleMode(enum.IntEnum):
     NONE = 0
     PER_HEAD = 1
     PER_BLOCK = 2
+    PER_TOKEN = 3
 
 
 class GGError(RuntimeError):
@@ -66,6 +68,7 @@ SIGNATURES = {
     "gg_kv_layer_bytes": (_sz, [_vp]),
     "gg_kv_set_head_scales": (_i, [_vp, _i, C.POINTER(_f), C.POINTER(_f)]),
     "gg_kv_append": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
+    "gg_kv_read": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
     "gg_kv_snapshot_bytes": (_sz, [_vp, _i]),
     "gg_kv_snapshot": (_i, [_vp, _vp, _i, _vp, _sz, _vp, _vp]),
     "gg_kv_restore": (_i, [_vp, _vp, _i, _vp, _sz, _vp, _vp]),

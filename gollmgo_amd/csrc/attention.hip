@@ -298,8 +298,9 @@ gg_status_t launch_verify_attention(const AttnArgs& a, hipStream_t s) {
             constexpr gg_dtype_t DT = decltype(dt_tag)::value;
             auto small = [&](auto dc_tag) {
                 constexpr int N = decltype(dc_tag)::value;
-                if (vrun && fused) attn_generic_kernel<DT, N, true, true><<<grid, threads, 0, s>>>(m, view);
-                else if (vrun) attn_generic_kernel<DT, N, true, false><<<grid, threads, 0, s>>>(m, view);
+                constexpr bool kRun = DT != GG_DTYPE_INT4;  // (4-bit V by element)
+                if (vrun && fused) attn_generic_kernel<DT, N, kRun, true><<<grid, threads, 0, s>>>(m, view);
+                else if (vrun) attn_generic_kernel<DT, N, kRun, false><<<grid, threads, 0, s>>>(m, view);
                 else if (fused) attn_generic_kernel<DT, N, false, true><<<grid, threads, 0, s>>>(m, view);
                 else attn_generic_kernel<DT, N, false, false><<<grid, threads, 0, s>>>(m, view);
             };
@@ -318,6 +319,7 @@ gg_status_t launch_verify_attention(const AttnArgs& a, hipStream_t s) {
             case GG_DTYPE_BF16: launch(std::integral_constant<gg_dtype_t, GG_DTYPE_BF16>{}); break;
             case GG_DTYPE_FP8_E4M3: launch(std::integral_constant<gg_dtype_t, GG_DTYPE_FP8_E4M3>{}); break;
             case GG_DTYPE_INT8: launch(std::integral_constant<gg_dtype_t, GG_DTYPE_INT8>{}); break;
+            case GG_DTYPE_INT4: launch(std::integral_constant<gg_dtype_t, GG_DTYPE_INT4>{}); break;
             default: return fail(GG_ERR_INVALID, "attention: pool dtype");
         }
     }

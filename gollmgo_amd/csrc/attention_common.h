@@ -1,6 +1,7 @@
 // attention_common.h — pool view and helpers shared by the attention kernels.
 #pragma once
 #include "gg_common.h"
+#include "int4.h"
 
 namespace gg {
 
@@ -16,6 +17,7 @@ struct KVView {
     const float* v_head_scale;
     const uint16_t* k_blk_scale;   // PER_BLOCK fp16 [blocks][Hkv]
     const uint16_t* v_blk_scale;
+    const uint32_t* words;         // PER_TOKEN [blocks][Hkv][bs] (int4.h)
     gg_dtype_t dt;
     int Hkv, D, bs;
     int num_blocks;  // block ids outside [0, num_blocks) read as empty
@@ -28,6 +30,7 @@ struct KVView {
             case GG_DTYPE_BF16: return bf16_bits_to_f32(((const uint16_t*)base)[i]);
             case GG_DTYPE_FP8_E4M3: return fp8e4m3_to_f32(base[i]);
             case GG_DTYPE_INT8: return (float)((const int8_t*)base)[i];
+            case GG_DTYPE_INT4: break;  // (k_value, v_value)
         }
         return 0.f;
     }
@@ -50,6 +53,22 @@ struct KVView {
         if (dt == GG_DTYPE_INT8) return f16_bits_to_f32(v_blk_scale[(size_t)blk * Hkv + h]);
         return 1.f;
     }
+    // The token word of (block, head, offset) of a 4-bit pool, and what element (token, d) of any
+    // pool stands for.
+    __device__ __forceinline__ uint32_t word(int blk, int h, int off) const { return words[((size_t)blk * Hkv + h) * bs + off]; }
+    __device__ __forceinline__ float k_value(int blk, int h, int off, int d) const {
+        if (dt != GG_DTYPE_INT4) return k_at(blk, h, off, d) * k_scale(blk, h);
+        const uint32_t w = word(blk, h, off);
+        const uint32_t b = kc[tile0(blk, h) / 2 + (size_t)off * (D / 2) + d / 2];
+        return int4_k_scale(w) * (float)((int)((d & 1) ? b >> 4 : b & 15u) - int4_k_zero(w));
+    }
+    __device__ __forceinline__ float v_value(int blk, int h, int off, int d) const {
+        if (dt != GG_DTYPE_INT4) return v_at(blk, h, off, d) * v_scale(blk, h);
+        const uint32_t w = word(blk, h, off);
+        const bool up = d >= D / 2;
+        const uint32_t b = vc[tile0(blk, h) / 2 + (size_t)(up ? d - D / 2 : d) * bs + off];
+        return int4_v_scale(w) * (float)((int)(up ? b >> 4 : b & 15u) - int4_v_zero(w));
+    }
 #endif
 };
 
@@ -63,6 +82,8 @@ inline KVView make_kv_view(const KV* kv, int layer) {
     } else if (kv->scale_mode == GG_SCALE_PER_BLOCK) {
         v.k_blk_scale = (const uint16_t*)kv->k_scales + (size_t)layer * kv->scale_layer_elems;
         v.v_blk_scale = (const uint16_t*)kv->v_scales + (size_t)layer * kv->scale_layer_elems;
+    } else if (kv->scale_mode == GG_SCALE_PER_TOKEN) {
+        v.words = (const uint32_t*)kv->k_scales + (size_t)layer * kv->scale_layer_elems;
     }
     v.dt = kv->dtype;
     v.Hkv = kv->num_kv_heads;
@@ -130,7 +151,7 @@ struct AttnShape {
 inline bool attn_full_supported(const KV* kv, int rows, int num_q_heads) {
     const long long tiles = ((long long)(num_q_heads / kv->num_kv_heads) * rows + 15) / 16;
     return kv->block_size == 16 && (kv->head_dim == 64 || (kv->head_dim == 128 && tiles > 4)) &&
-           kv->dtype != GG_DTYPE_F32 && kv->num_kv_heads * tiles <= 0x7fff;
+           kv->dtype != GG_DTYPE_F32 && kv->dtype != GG_DTYPE_INT4 && kv->num_kv_heads * tiles <= 0x7fff;
 }
 inline AttnShape attn_shape(const KV* kv, int rows, int num_q_heads) {
     const int tiles = (num_q_heads / kv->num_kv_heads * rows + 15) / 16;
@@ -419,6 +440,21 @@ __device__ __forceinline__ void append_int8_run(const AttnArgs& a, const KVView&
     }
 }
 
+// 4-bit pools: rows [j0, j1) of item (b, kvh), a row per wave, with gg_kv_append's rule.
+__device__ __forceinline__ void append_int4_rows(const AttnArgs& a, const KVView& kv, int b, int kvh, int ctx, int nrows,
+                                                 int j0, int j1) {
+    const Int4View p{const_cast<uint8_t*>(kv.kc), const_cast<uint8_t*>(kv.vc), const_cast<uint32_t*>(kv.words), kv.Hkv, kv.D,
+                     kv.bs, (long long)kv.num_blocks * kv.bs};
+    for (int j = j0 + (int)(threadIdx.x >> 6); j < j1; j += blockDim.x >> 6) {
+        const int pos = ctx - nrows + j;
+        const int blk = a.block_tables[(size_t)b * a.max_blocks + pos / kv.bs];
+        if (blk < 0 || blk >= kv.num_blocks) continue;
+        const size_t at = (((size_t)b * a.rows + j) * kv.Hkv + kvh) * kv.D;
+        int4_write_row(p, blk, kvh, pos % kv.bs, [&](int d) { return load_as_f32(a.k_new, a.new_dtype, at + d); },
+                       [&](int d) { return load_as_f32(a.v_new, a.new_dtype, at + d); });
+    }
+}
+
 // Rows [j0, j1) of item (b, kvh) (clamped to the sequence's rows), by a whole workgroup,
 // before anything reads them. PER_BLOCK INT8 pools go block by block (append_int8_run).
 __device__ __forceinline__ void append_item_rows(const AttnArgs& a, const KVView& kv, int b, int kvh, int j0 = 0,
@@ -428,6 +464,10 @@ __device__ __forceinline__ void append_item_rows(const AttnArgs& a, const KVView
     if (ctx <= 0 || nrows <= 0 || nrows > ctx) return;
     j0 = j0 < 0 ? 0 : j0;
     j1 = j1 > nrows ? nrows : j1;
+    if (kv.dt == GG_DTYPE_INT4) {
+        append_int4_rows(a, kv, b, kvh, ctx, nrows, j0, j1);
+        return;
+    }
     if (kv.dt == GG_DTYPE_INT8) {
         for (int j = j0; j < j1;) {
             const int pos = ctx - nrows + j;

@@ -15,13 +15,17 @@ __device__ __forceinline__ float pool_elem(const uint8_t* base, size_t i) {
     else if constexpr (DT == GG_DTYPE_F16) return f16_bits_to_f32(((const uint16_t*)base)[i]);
     else if constexpr (DT == GG_DTYPE_BF16) return bf16_bits_to_f32(((const uint16_t*)base)[i]);
     else if constexpr (DT == GG_DTYPE_FP8_E4M3) return fp8e4m3_to_f32(base[i]);
+    else if constexpr (DT == GG_DTYPE_INT4) return (float)((base[i >> 1] >> (4 * (i & 1))) & 15u);
     else return (float)((const int8_t*)base)[i];
 }
 
 // The pool elements in 16 bytes, as f32.
 template <gg_dtype_t DT>
 struct Pool16 {
-    static constexpr int kN = DT == GG_DTYPE_F32 ? 4 : (DT == GG_DTYPE_F16 || DT == GG_DTYPE_BF16) ? 8 : 16;
+    static constexpr int kN = DT == GG_DTYPE_F32                              ? 4
+                              : (DT == GG_DTYPE_F16 || DT == GG_DTYPE_BF16) ? 8
+                              : DT == GG_DTYPE_INT4                         ? 32
+                                                                            : 16;
     __device__ static __forceinline__ void decode(const uint4 r, float (&f)[kN]) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -34,6 +38,7 @@ struct Pool16 {
                        : (k & 3) == 1 ? fp8e4m3_to_f32<1>(w[k >> 2])
                        : (k & 3) == 2 ? fp8e4m3_to_f32<2>(w[k >> 2])
                                       : fp8e4m3_to_f32<3>(w[k >> 2]);
+            else if constexpr (DT == GG_DTYPE_INT4) f[k] = (float)((w[k >> 3] >> (4 * (k & 7))) & 15u);
             else f[k] = (float)(int8_t)(uint8_t)(w[k >> 2] >> (8 * (k & 3)));
         }
     }
@@ -49,6 +54,8 @@ struct Pool16 {
 // line per lane and key) and the merge in a launch, 4 x 5 rows of 8 heads over 64-256 fp32 keys
 // took 14.0 + 4.2 µs, now 8.8; per call on one box, four fp32 sequences of 100-700 keys at
 // head_dim 128 64 -> 25 µs, eight bf16 ones at head_dim 96 132 -> 24.
+// 4-bit pools: codes less their token's zero point, its scales on the score and on p (no V runs:
+// a run of a 16-token block is 8 bytes of two dims each).
 template <gg_dtype_t DT, int DC, bool kVRun>
 __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVView& kv, int b, int kvh, int t0, int t1,
                                                   const float* s_q, float* s_p, size_t* s_vrow, float (&acc)[DC], float& m,
@@ -57,6 +64,8 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
     const int D = kv.D;
     const int32_t* bt = a.block_tables + (size_t)b * a.max_blocks;
     const uint8_t* vc = kv.vc;
+    constexpr bool kInt4 = DT == GG_DTYPE_INT4;
+    static_assert(!(kInt4 && kVRun), "4-bit V by element");
     constexpr int kN = Pool16<DT>::kN;
     constexpr int kRuns = 64 / kN;  // 16-byte V runs of a tile per dim
     m = -1e30f;
@@ -73,7 +82,12 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
             if (blk < 0 || blk >= kv.num_blocks) blk = -1;  // invalid table entry: key skipped
         }
         // (Skipped keys read block 0.)
-        const size_t vrow = kv.tile0(max(blk, 0), kvh) + off;
+        const size_t vrow = kInt4 ? kv.tile0(max(blk, 0), kvh) / 2 + off : kv.tile0(max(blk, 0), kvh) + off;
+        [[maybe_unused]] uint32_t word = 0;
+        if constexpr (kInt4) {
+            if (blk >= 0) word = kv.word(blk, kvh, off);
+        }
+        [[maybe_unused]] const float kzero = kInt4 ? (float)int4_k_zero(word) : 0.f;
         [[maybe_unused]] uint4 vr[kVRun ? DC : 1][kVRun ? kRuns : 1];
         if constexpr (kVRun) {
 #pragma unroll
@@ -91,7 +105,8 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
         if (blk >= 0) {
             // The lane's key row is contiguous: 16-byte loads when rows are whole
             // multiples of 16 bytes (pools are 256-byte aligned), else element loads.
-            const uint8_t* krow = kv.kc + (kv.tile0(blk, kvh) + (size_t)off * D) * dtype_bytes(DT);
+            const size_t krow_i = kv.tile0(blk, kvh) + (size_t)off * D;
+            const uint8_t* krow = kv.kc + (kInt4 ? krow_i / 2 : krow_i * dtype_bytes(DT));
             float dot = 0.f;
             if (D % kN == 0) {
 #pragma unroll(DT == GG_DTYPE_F32 ? 16 : 4)
@@ -99,13 +114,14 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
                     float f[kN];
                     Pool16<DT>::decode(((const uint4*)krow)[v], f);
 #pragma unroll
-                    for (int e = 0; e < kN; ++e) dot += s_q[v * kN + e] * f[e];
+                    for (int e = 0; e < kN; ++e) dot += s_q[v * kN + e] * (kInt4 ? f[e] - kzero : f[e]);
                 }
             } else {
 #pragma unroll 16
-                for (int d = 0; d < D; ++d) dot += s_q[d] * pool_elem<DT>(krow, d);
+                for (int d = 0; d < D; ++d)
+                    dot += s_q[d] * (kInt4 ? pool_elem<DT>(krow, d) - kzero : pool_elem<DT>(krow, d));
             }
-            sc = dot * a.scale * kv.k_scale(blk, kvh);
+            sc = dot * a.scale * (kInt4 ? int4_k_scale(word) : kv.k_scale(blk, kvh));
         }
         float mt = sc;
         for (int o = 32; o > 0; o >>= 1) mt = fmaxf(mt, __shfl_xor(mt, o));
@@ -122,8 +138,9 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
         // below has no cross-lane operations. (Masked and skipped keys have p = 0.)
         // One wave's own slots: its LDS operations complete in order.
         __builtin_amdgcn_wave_barrier();
-        s_p[lane] = blk >= 0 ? p * kv.v_scale(blk, kvh) : 0.f;
-        if constexpr (!kVRun) s_vrow[lane] = vrow;
+        s_p[lane] = blk >= 0 ? p * (kInt4 ? int4_v_scale(word) : kv.v_scale(blk, kvh)) : 0.f;
+        if constexpr (kInt4) s_vrow[lane] = vrow | ((size_t)int4_v_zero(word) << 60);  // (pools are far below 2^60 bytes)
+        else if constexpr (!kVRun) s_vrow[lane] = vrow;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -150,7 +167,13 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
                     const int d = lane + 64 * c;
-                    if (d < D) acc[c] += pi * pool_elem<DT>(vc, vr0 + (size_t)d * kv.bs);
+                    if constexpr (kInt4) {
+                        const bool up = d >= D / 2;
+                        const uint8_t* q = vc + (vr0 & (((size_t)1 << 60) - 1)) + (size_t)(up ? d - D / 2 : d) * kv.bs;
+                        if (d < D) acc[c] += pi * ((float)((*q >> (up ? 4 : 0)) & 15u) - (float)(int)(vr0 >> 60));
+                    } else if (d < D) {
+                        acc[c] += pi * pool_elem<DT>(vc, vr0 + (size_t)d * kv.bs);
+                    }
                 }
             }
         }

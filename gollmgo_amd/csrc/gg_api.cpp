@@ -69,11 +69,14 @@ GG_API gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size, 
                      head_dim > 0,
                  "gg_kv_create: sizes must be positive");
     GG_CHECK_ARG(head_dim <= 1024, "gg_kv_create: head_dim must be <= 1024");
-    GG_CHECK_ARG(dtype_bytes(dtype) != 0, "gg_kv_create: unknown dtype");
+    GG_CHECK_ARG(dtype_bytes(dtype) != 0 || dtype == GG_DTYPE_INT4, "gg_kv_create: unknown dtype");
     if (dtype == GG_DTYPE_FP8_E4M3) {
         GG_CHECK_ARG(scale_mode == GG_SCALE_PER_HEAD, "gg_kv_create: FP8 pools need GG_SCALE_PER_HEAD");
     } else if (dtype == GG_DTYPE_INT8) {
         GG_CHECK_ARG(scale_mode == GG_SCALE_PER_BLOCK, "gg_kv_create: INT8 pools need GG_SCALE_PER_BLOCK");
+    } else if (dtype == GG_DTYPE_INT4) {
+        GG_CHECK_ARG(scale_mode == GG_SCALE_PER_TOKEN, "gg_kv_create: INT4 pools need GG_SCALE_PER_TOKEN");
+        GG_CHECK_ARG(head_dim % 2 == 0, "gg_kv_create: INT4 pools need an even head_dim");
     } else {
         GG_CHECK_ARG(scale_mode == GG_SCALE_NONE, "gg_kv_create: float pools take GG_SCALE_NONE");
     }
@@ -98,8 +101,7 @@ GG_API gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size, 
     kv->head_dim = head_dim;
     kv->dtype = dtype;
     kv->scale_mode = scale_mode;
-    kv->elem_bytes = dtype_bytes(dtype);
-    kv->tile_bytes = (size_t)block_size * head_dim * kv->elem_bytes;
+    kv->tile_bytes = kv_tile_bytes(dtype, block_size, head_dim);
     kv->layer_bytes = (size_t)num_blocks * num_kv_heads * kv->tile_bytes;
     kv->layer_stride = 2 * kv->layer_bytes;
     (void)hipGetDevice(&kv->device);
@@ -127,6 +129,13 @@ GG_API gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size, 
         if (st == GG_OK) st = check_hip(hipMalloc(&kv->v_scales, b), "hipMalloc(V scales)");
         if (st == GG_OK) st = check_hip(hipMemset(kv->k_scales, 0, b), "scales init");
         if (st == GG_OK) st = check_hip(hipMemset(kv->v_scales, 0, b), "scales init");
+    }
+    if (st == GG_OK && scale_mode == GG_SCALE_PER_TOKEN) {
+        // A word of 0 is a scale of 0: slots never written hold zeros.
+        kv->scale_layer_elems = (size_t)num_blocks * num_kv_heads * block_size;
+        size_t b = kv->scale_layer_elems * num_layers * sizeof(uint32_t);
+        st = check_hip(hipMalloc(&kv->k_scales, b), "hipMalloc(token scales)");
+        if (st == GG_OK) st = check_hip(hipMemset(kv->k_scales, 0, b), "scales init");
     }
     if (st != GG_OK) {
         std::string msg = t_last_error;
@@ -161,11 +170,14 @@ GG_API void* gg_kv_v_layer_ptr(gg_kv_t kv, int layer) {
 }
 static void* scale_ptr(gg_kv_t kv, void* base, int layer) {
     if (!kv || !base || layer < 0 || layer >= kv->num_layers) return nullptr;
-    size_t eb = kv->scale_mode == GG_SCALE_PER_HEAD ? sizeof(float) : sizeof(uint16_t);
+    size_t eb = kv->scale_mode == GG_SCALE_PER_BLOCK ? sizeof(uint16_t) : sizeof(float);
     return (uint8_t*)base + (size_t)layer * kv->scale_layer_elems * eb;
 }
 GG_API void* gg_kv_k_scale_ptr(gg_kv_t kv, int layer) { return kv ? scale_ptr(kv, kv->k_scales, layer) : nullptr; }
-GG_API void* gg_kv_v_scale_ptr(gg_kv_t kv, int layer) { return kv ? scale_ptr(kv, kv->v_scales, layer) : nullptr; }
+GG_API void* gg_kv_v_scale_ptr(gg_kv_t kv, int layer) {
+    if (!kv) return nullptr;
+    return scale_ptr(kv, kv->scale_mode == GG_SCALE_PER_TOKEN ? kv->k_scales : kv->v_scales, layer);
+}
 GG_API size_t gg_kv_layer_bytes(gg_kv_t kv) { return kv ? kv->layer_bytes : 0; }
 
 GG_API gg_status_t gg_kv_set_head_scales(gg_kv_t kv, int layer, const float* k_scales,
@@ -237,6 +249,18 @@ GG_API gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void
     GG_CHECK_ARG(is_float_io(src_dtype), "gg_kv_append: src dtype must be F32/F16/BF16");
     GG_CHECK_ARG(n_rows <= (1 << 24), "gg_kv_append: n_rows too large");
     return launch_kv_append(kv, layer, k, v, src_dtype, slot_mapping, n_rows, (hipStream_t)stream);
+}
+
+GG_API gg_status_t gg_kv_read(gg_kv_t kv, int layer, void* k_out, void* v_out, gg_dtype_t out_dtype,
+                              const int32_t* slot_mapping, int n_rows, void* stream) {
+    clear_error();
+    GG_CHECK_ARG(kv != nullptr, "gg_kv_read: kv is NULL");
+    GG_CHECK_ARG(layer >= 0 && layer < kv->num_layers, "gg_kv_read: layer out of range");
+    GG_CHECK_ARG(n_rows >= 0 && n_rows <= (1 << 24), "gg_kv_read: n_rows out of range");
+    GG_CHECK_ARG(is_float_io(out_dtype), "gg_kv_read: out dtype must be F32/F16/BF16");
+    if (n_rows == 0) return GG_OK;
+    GG_CHECK_ARG(slot_mapping && (k_out || v_out), "gg_kv_read: NULL buffer");
+    return launch_kv_read(kv, layer, k_out, v_out, out_dtype, slot_mapping, n_rows, (hipStream_t)stream);
 }
 
 // ---------------------------------------------------------------- attention

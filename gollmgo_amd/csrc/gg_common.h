@@ -28,14 +28,15 @@ struct KV {
     gg_dtype_t dtype = GG_DTYPE_BF16;
     gg_scale_mode_t scale_mode = GG_SCALE_NONE;
     int device = 0;
-    size_t elem_bytes = 2;
     size_t layer_bytes = 0;       // bytes of one layer's K (or V) pool
     size_t tile_bytes = 0;        // one (block, head) tile of K (or V): block_size * head_dim elements
     size_t layer_stride = 0;      // bytes between layers (K and V interleaved: 2 * layer_bytes)
     size_t scale_layer_elems = 0; // scales per layer per pool
     uint8_t* k_pool = nullptr;    // [layers][blocks][heads][K tile, V tile]: the allocation
     uint8_t* v_pool = nullptr;    // k_pool + tile_bytes (inside that allocation)
-    void* k_scales = nullptr;     // PER_HEAD: float[layers][Hkv]; PER_BLOCK: u16[layers][blocks][Hkv]
+    // PER_HEAD: float[layers][Hkv]; PER_BLOCK: u16[layers][blocks][Hkv]; PER_TOKEN:
+    // u32[layers][blocks][Hkv][block_size] for both, in k_scales
+    void* k_scales = nullptr;
     void* v_scales = nullptr;
 };
 
@@ -46,8 +47,15 @@ __host__ __device__ inline size_t dtype_bytes(gg_dtype_t t) {
         case GG_DTYPE_BF16: return 2;
         case GG_DTYPE_FP8_E4M3: return 1;
         case GG_DTYPE_INT8: return 1;
+        case GG_DTYPE_INT4: return 0;  // (half a byte: kv_tile_bytes)
     }
     return 0;
+}
+
+// Bytes of one (block, head) tile of K (or V).
+inline size_t kv_tile_bytes(gg_dtype_t t, int block_size, int head_dim) {
+    const size_t n = (size_t)block_size * head_dim;
+    return t == GG_DTYPE_INT4 ? n / 2 : n * dtype_bytes(t);
 }
 
 __host__ __device__ inline bool is_float_io(gg_dtype_t t) {
@@ -61,6 +69,10 @@ gg_status_t launch_kv_restore(KV* kv, const int32_t* ids, int n, void* staging, 
                               hipStream_t s);
 gg_status_t launch_kv_append(KV* kv, int layer, const void* k, const void* v, gg_dtype_t src,
                              const int32_t* slots, int n_rows, hipStream_t s);
+gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* v, gg_dtype_t src, const int32_t* slots,
+                                  int n_rows, hipStream_t s);
+gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype_t dst, const int32_t* slots, int n_rows,
+                           hipStream_t s);
 
 struct AttnArgs {
     const KV* kv;

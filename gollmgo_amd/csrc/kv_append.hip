@@ -645,6 +645,7 @@ void launch_run(const AppendArgs& a, hipStream_t s) {
 gg_status_t launch_kv_append(KV* kv, int layer, const void* k, const void* v, gg_dtype_t src,
                              const int32_t* slots, int n_rows, hipStream_t s) {
     if (n_rows == 0) return GG_OK;
+    if (kv->dtype == GG_DTYPE_INT4) return launch_kv_append_int4(kv, layer, k, v, src, slots, n_rows, s);
     AppendArgs a{};
     a.kc = kv->k_pool + (size_t)layer * kv->layer_stride;
     a.vc = kv->v_pool + (size_t)layer * kv->layer_stride;

@@ -8,8 +8,8 @@
 //
 // A (block, layer) record is the block's tiles of that layer — for every kv head its K
 // tile then its V tile, already adjacent in the pool — followed, for PER_BLOCK INT8
-// pools, by the block's fp16 K and V scales of that layer (2 * Hkv values), the record
-// padded to 16 bytes. Records are ordered [block i][layer]. PER_HEAD scales belong to the
+// pools, by the block's fp16 K and V scales of that layer (2 * Hkv values), for PER_TOKEN
+// INT4 pools by its tokens' scale words (Hkv * block_size), the record padded to 16 bytes. Records are ordered [block i][layer]. PER_HEAD scales belong to the
 // layer, not to a block, and stay with the pool.
 #include "gg_common.h"
 
@@ -20,11 +20,13 @@ struct SwapArgs {
     uint8_t* pool;          // the KV allocation (layer 0, block 0, head 0, K tile)
     uint16_t* k_bscale;     // PER_BLOCK scales (layer 0) or NULL
     uint16_t* v_bscale;
+    uint32_t* words;        // PER_TOKEN words (layer 0) or NULL
+    int block_words;        // Hkv * block_size
     const int32_t* ids;
     int n, layers, num_blocks, Hkv;
     size_t tiles_bytes;     // Hkv * 2 * tile: one block's tiles of one layer
     size_t layer_stride;    // bytes between layers in the pool
-    size_t scale_layer;     // scales per layer (blocks * Hkv)
+    size_t scale_layer;     // scales (words) per layer
     size_t record;          // bytes of one (block, layer) record
     uint8_t* staging;
 };
@@ -55,6 +57,14 @@ __global__ void __launch_bounds__(256) swap_kernel(SwapArgs a) {
             }
         }
     }
+    if (a.words) {
+        uint32_t* rw = (uint32_t*)(rec + (a.tiles_bytes + 3) / 4 * 4);
+        uint32_t* w = a.words + (size_t)layer * a.scale_layer + (size_t)(ok ? blk : 0) * a.block_words;
+        for (int k = threadIdx.x; k < a.block_words; k += blockDim.x) {
+            if (!RESTORE) rw[k] = ok ? w[k] : 0u;
+            else if (ok) w[k] = rw[k];
+        }
+    }
     if (a.k_bscale) {
         uint16_t* rs = (uint16_t*)(rec + a.tiles_bytes);
         const size_t base = (size_t)layer * a.scale_layer + (size_t)(ok ? blk : 0) * a.Hkv;
@@ -79,6 +89,10 @@ SwapArgs swap_args(KV* kv, const int32_t* ids, int n, void* staging) {
         a.k_bscale = (uint16_t*)kv->k_scales;
         a.v_bscale = (uint16_t*)kv->v_scales;
     }
+    if (kv->scale_mode == GG_SCALE_PER_TOKEN) {
+        a.words = (uint32_t*)kv->k_scales;
+        a.block_words = kv->num_kv_heads * kv->block_size;
+    }
     a.ids = ids;
     a.n = n;
     a.layers = kv->num_layers;
@@ -97,6 +111,7 @@ SwapArgs swap_args(KV* kv, const int32_t* ids, int n, void* staging) {
 size_t kv_swap_record_bytes(const KV* kv) {
     size_t r = (size_t)kv->num_kv_heads * 2 * kv->tile_bytes;
     if (kv->scale_mode == GG_SCALE_PER_BLOCK) r += (size_t)kv->num_kv_heads * 2 * sizeof(uint16_t);
+    if (kv->scale_mode == GG_SCALE_PER_TOKEN) r = (r + 3) / 4 * 4 + (size_t)kv->num_kv_heads * kv->block_size * sizeof(uint32_t);
     return (r + 15) / 16 * 16;
 }
 

@@ -6,6 +6,7 @@ of libgg_verify.so. Names follow the reference's domain:
 
   KVCache            ~ CUDAKVCache (internal/backend/cuda/kvcache_bridge.go:16-91)
   KVCache.append     ~ CUDAKVCache.Write / gollmgo_kvcache_write
+  KVCache.read       (none) rows of a pool as numbers
   KVCache.attention  ~ gollmgo_kvcache_attention, for k+1 verify rows per sequence
   accept_greedy      ~ Verify + argmax as emitSpeculative drives them
                        (internal/engine/speculative.go:68-84, serving.go:514-566)
@@ -61,7 +62,7 @@ class _DeviceBuffer:
         }
 
 
-_ELEM_BYTES = {DType.F32: 4, DType.F16: 2, DType.BF16: 2, DType.FP8_E4M3: 1, DType.INT8: 1}
+_ELEM_BITS = {DType.F32: 32, DType.F16: 16, DType.BF16: 16, DType.FP8_E4M3: 8, DType.INT8: 8, DType.INT4: 4}
 
 
 def device_bytes(ptr: int, nbytes: int) -> torch.Tensor:
@@ -71,13 +72,16 @@ def device_bytes(ptr: int, nbytes: int) -> torch.Tensor:
 
 class KVCache:
     """Paged K/V pools for all layers (K[blk][Hkv][bs][D], V[blk][Hkv][D][bs]; in device
-    memory the K and V tiles of each (block, head) are adjacent)."""
+    memory the K and V tiles of each (block, head) are adjacent). INT4 pools hold two codes to
+    a byte, K[blk][Hkv][bs][D/2] (byte i: dims 2i, 2i+1) and V[blk][Hkv][D/2][bs] (byte i: dims
+    i, i+D/2), the first in the low half."""
 
     def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int,
                  head_dim: int, dtype: DType):
         self.num_layers, self.num_blocks, self.block_size = num_layers, num_blocks, block_size
         self.num_kv_heads, self.head_dim, self.dtype = num_kv_heads, head_dim, DType(dtype)
-        self.scale_mode = {DType.FP8_E4M3: ScaleMode.PER_HEAD, DType.INT8: ScaleMode.PER_BLOCK}.get(
+        self.scale_mode = {DType.FP8_E4M3: ScaleMode.PER_HEAD, DType.INT8: ScaleMode.PER_BLOCK,
+                           DType.INT4: ScaleMode.PER_TOKEN}.get(
             self.dtype, ScaleMode.NONE)
         torch.cuda.init()
         h = C.c_void_p()
@@ -104,7 +108,7 @@ class KVCache:
     def _pool(self, ptr: int) -> torch.Tensor:
         # The K and V tiles of each (block, head) alternate in device memory; gather one
         # pool's tiles into its logical [blocks][heads][tile] bytes (a device copy).
-        tile = self.block_size * self.head_dim * _ELEM_BYTES[self.dtype]
+        tile = self.block_size * self.head_dim * _ELEM_BITS[self.dtype] // 8
         n = self.num_blocks * self.num_kv_heads
         raw = device_bytes(ptr, (2 * n - 1) * tile)
         return torch.as_strided(raw, (n, tile), (2 * tile, 1)).reshape(-1)
@@ -118,7 +122,14 @@ class KVCache:
         return self._pool(lib().gg_kv_v_layer_ptr(self.handle, layer))
 
     def scales(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """(k, v) scales: PER_HEAD fp32 [Hkv]; PER_BLOCK fp16 [blocks, Hkv]."""
+        """(k, v) scales: PER_HEAD fp32 [Hkv]; PER_BLOCK fp16 [blocks, Hkv]; PER_TOKEN (scale
+        fp32, zero point int32) of each [blocks, Hkv, bs], copies taken from the packed words."""
+        if self.scale_mode == ScaleMode.PER_TOKEN:
+            n = self.num_blocks * self.num_kv_heads * self.block_size
+            w = device_bytes(lib().gg_kv_k_scale_ptr(self.handle, layer), n * 4).view(torch.int32)
+            w = w.view(self.num_blocks, self.num_kv_heads, self.block_size)
+            half = lambda h: (((h & 0xfff0) << 15).view(torch.float32), h & 15)
+            return half(w & 0xffff), half((w >> 16) & 0xffff)
         if self.scale_mode == ScaleMode.PER_HEAD:
             n, dt = self.num_kv_heads * 4, torch.float32
         elif self.scale_mode == ScaleMode.PER_BLOCK:
@@ -144,6 +155,28 @@ class KVCache:
         check(lib().gg_kv_append(self.handle, layer, _dev(k, "k"), _dev(v, "v", k.dtype), int(dtype_of(k)),
                                  _dev(slot_mapping, "slot_mapping", torch.int32), n, _stream(stream)),
               "gg_kv_append")
+
+    def read(self, layer: int, slot_mapping: torch.Tensor, dtype: Optional[torch.dtype] = None,
+             out: Optional[tuple] = None, stream: Optional[torch.cuda.Stream] = None):
+        """The rows in `slot_mapping` as numbers (gg_kv_read): (k, v), each
+        [n_rows, num_kv_heads, head_dim] of `dtype` (bfloat16 unless given), or written to
+        out = (k, v), of which one may be None. Rows whose slot is negative or past the pool
+        are left as they were (in new tensors: not set)."""
+        n = int(slot_mapping.numel())
+        if out is None:
+            k, v = (torch.empty(n, self.num_kv_heads, self.head_dim, dtype=dtype or torch.bfloat16,
+                                device=slot_mapping.device) for _ in range(2))
+        else:
+            k, v = out
+        given = [t for t in (k, v) if t is not None]
+        if not given or any(t.numel() != n * self.num_kv_heads * self.head_dim for t in given):
+            raise ValueError("k/v must be [n_rows, num_kv_heads, head_dim] matching slot_mapping")
+        if any(t.dtype != given[0].dtype or (dtype is not None and t.dtype != dtype) for t in given):
+            raise TypeError("k and v must share one dtype")
+        check(lib().gg_kv_read(self.handle, layer, _dev(k, "k") if k is not None else None,
+                               _dev(v, "v") if v is not None else None, int(dtype_of(given[0])),
+                               _dev(slot_mapping, "slot_mapping", torch.int32), n, _stream(stream)), "gg_kv_read")
+        return k, v
 
     def snapshot_bytes(self, num_blocks: int) -> int:
         return lib().gg_kv_snapshot_bytes(self.handle, num_blocks)

@@ -27,6 +27,11 @@
  *   2 * tile bytes apart (tile = block_size * head_dim * element bytes), likewise V.
  * A reference slot index (internal/kvcache/block_table.go:39) still addresses a
  * token: slot = physical_block * block_size + offset.
+ *
+ * INT4 pools (head_dim even) hold two codes to a byte, and no byte holds two tokens:
+ *   K tile: [block_size][head_dim / 2], byte i = dims 2i (low half) and 2i + 1
+ *   V tile: [head_dim / 2][block_size], byte (i, t) = dims i (low half) and
+ *           i + head_dim / 2 of token t
  */
 #ifndef GG_VERIFY_H
 #define GG_VERIFY_H
@@ -54,6 +59,7 @@ typedef enum {
     GG_DTYPE_BF16 = 2,
     GG_DTYPE_FP8_E4M3 = 3,
     GG_DTYPE_INT8 = 4,
+    GG_DTYPE_INT4 = 5, /* pools only: 4-bit codes, two to a byte */
 } gg_dtype_t;
 
 /* How a quantised KV pool is scaled (dequant: x = q * scale).
@@ -62,11 +68,23 @@ typedef enum {
  *              kernels/gollmgo_model.cu:415-427, applied per head).
  *   PER_BLOCK: one fp16 scale per (layer, block, kv head) for K and for V,
  *              maintained by gg_kv_append as the running amax/127 of the block
- *              (int8 convention of kernels/gollmgo_model.cu:430-441). */
+ *              (int8 convention of kernels/gollmgo_model.cu:430-441).
+ *   PER_TOKEN: INT4 pools. A scale s and a zero point z per (layer, token, kv head), for K
+ *              and for V apart: codes n in 0..15 stand for s * (n - z). Of a row x of
+ *              head_dim values (in fp32; NaN taken as 0, magnitudes past 1e36 as 1e36):
+ *                lo = min(0, min x), hi = max(0, max x)
+ *                s  = (hi - lo) / 15, rounded up to five significant bits, at least 2^-100
+ *                z  = rint(-lo / s), n = rint(x / s) + z clamped to 0..15 (ties to even)
+ *              so zero is held exactly and no value moves by more than s / 2. A row
+ *              depends on itself alone: rows may come in any order and any slots.
+ *              Both scales and zero points take one 32-bit word per (token, kv head):
+ *              K in the low half, V in the high half, each half = the top 12 bits of s
+ *              after its sign (fp32 bits 30..19) << 4 | z. */
 typedef enum {
     GG_SCALE_NONE = 0,
     GG_SCALE_PER_HEAD = 1,
     GG_SCALE_PER_BLOCK = 2,
+    GG_SCALE_PER_TOKEN = 3,
 } gg_scale_mode_t;
 
 typedef struct gg_kv* gg_kv_t;
@@ -100,7 +118,9 @@ gg_status_t gg_kv_destroy(gg_kv_t kv);
  * arguments); tiles of one pool follow every 2 * tile bytes. */
 void* gg_kv_k_layer_ptr(gg_kv_t kv, int layer);
 void* gg_kv_v_layer_ptr(gg_kv_t kv, int layer);
-/* PER_HEAD: float[num_kv_heads]; PER_BLOCK: uint16 (fp16 bits)[num_blocks][num_kv_heads]. */
+/* PER_HEAD: float[num_kv_heads]; PER_BLOCK: uint16 (fp16 bits)[num_blocks][num_kv_heads];
+ * PER_TOKEN: uint32[num_blocks][num_kv_heads][block_size], one array for K and V (both
+ * calls return it). */
 void* gg_kv_k_scale_ptr(gg_kv_t kv, int layer);
 void* gg_kv_v_scale_ptr(gg_kv_t kv, int layer);
 /* Bytes of one layer's K (or V) tiles (num_blocks * num_kv_heads * tile); a layer
@@ -111,7 +131,7 @@ size_t gg_kv_layer_bytes(gg_kv_t kv);
  * (internal/backend/cuda/swap_bridge.go:53-153; interface internal/backend/runner.go:
  * 94-106). A snapshot of num_blocks blocks holds, for block i of block_ids (device
  * int32[num_blocks]) and every layer, that block's K and V tiles of all kv heads (plus
- * its fp16 K/V scales for PER_BLOCK pools), as gg_kv_snapshot_bytes(kv, num_blocks)
+ * its fp16 K/V scales for PER_BLOCK pools, its tokens' words for PER_TOKEN ones), as gg_kv_snapshot_bytes(kv, num_blocks)
  * bytes ordered [block i][layer]; PER_HEAD scales stay with the pool.
  *   gg_kv_snapshot: gathers the blocks into `staging` (device, 16-byte aligned, at least
  *                   gg_kv_snapshot_bytes) and, if host_dst is not NULL, copies it there
@@ -133,7 +153,7 @@ gg_status_t gg_kv_set_head_scales(gg_kv_t kv, int layer, const float* k_scales,
                                   const float* v_scales);
 
 /* Draft-KV append: write n_rows new K/V rows of one layer into their slots,
- * quantising on write for FP8/INT8 pools.
+ * quantising on write for FP8/INT8/INT4 pools.
  * Replaces gollmgo_kvcache_write (kernels/gollmgo_kvcache.h:41-45) and the
  * paged_kv_write_{f16,bf16} kernels (kernels/gollmgo_paged_attn.cu:14-35,126-146).
  *   k, v         : device [n_rows][num_kv_heads][head_dim] of src_dtype (F32/F16/BF16)
@@ -149,6 +169,15 @@ gg_status_t gg_kv_set_head_scales(gg_kv_t kv, int layer, const float* k_scales,
 gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void* v,
                          gg_dtype_t src_dtype, const int32_t* slot_mapping,
                          int n_rows, void* stream);
+
+/* Read rows of one layer back as numbers: row i of k_out / v_out (device
+ * [n_rows][num_kv_heads][head_dim] of out_dtype F32/F16/BF16; either may be NULL) is what
+ * the pool holds in slot_mapping[i], its scales applied in fp32 and rounded once. For
+ * kernels that take dense K/V, and to look at a cache. A row whose slot is negative or
+ * past the pool is left as it was. The inverse of gg_kv_append in its arguments; no
+ * counterpart in the reference (whose pools hold the source type). */
+gg_status_t gg_kv_read(gg_kv_t kv, int layer, void* k_out, void* v_out, gg_dtype_t out_dtype,
+                       const int32_t* slot_mapping, int n_rows, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Multi-query paged attention over the k+1 verify rows (split-K "v2").
