@@ -191,6 +191,15 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
                    int partition_tokens) {
     if (partition_tokens > 0) return {ATTN_SCHED_GRID, partition_tokens};
     const AttnShape sh = attn_shape(kv, rows, num_q_heads);
+    if (kv->dtype == GG_DTYPE_INT4) {
+        // A workgroup per item where the plan would cut nothing (tables below the shortest piece) or
+        // cannot rank the batch.
+        if (!sh.full || (long long)num_seqs * kv->num_kv_heads * sh.groups > 0x7fffffffLL)
+            return {ATTN_SCHED_GRID, attn_generic_partition(kv, num_seqs, rows, num_q_heads, max_blocks)};
+        const bool narrow = (long long)max_blocks * kv->block_size <= 64 * lpt_min_chunks(64);
+        const bool ranked = num_seqs <= kLptMaxSeqs && (long long)num_seqs * kv->num_kv_heads * sh.groups <= (1 << 18);
+        return {narrow || !ranked ? ATTN_SCHED_ITEMS : ATTN_SCHED_LPT, 0};
+    }
     // (2^18 heads over all sequences: a plan of a few MB.)
     if (sh.full && num_seqs <= kLptMaxSeqs && (long long)num_seqs * kv->num_kv_heads * sh.groups <= (1 << 18))
         return {ATTN_SCHED_LPT, 0};
@@ -207,7 +216,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
     // Past kLptMaxSeqs sequences: one workgroup per item, or stream-K where contexts are long.
     const long long max_keys = (long long)max_blocks * kv->block_size;
     const long long items = (long long)num_seqs * kv->num_kv_heads;
-    const long long slots = (long long)device_cu_count() * attn_occupancy((int)dtype_bytes(kv->dtype), sh.nt, kv->head_dim);
+    const long long slots = (long long)device_cu_count() * attn_kv_occupancy(kv, sh.nt);
     if (num_seqs <= kLptMaxSeqs) return {ATTN_SCHED_LPT, 0};
     if (items >= slots && max_keys <= kMfmaMaxPartition)
         return {ATTN_SCHED_GRID, (int)((max_keys + 63) / 64 * 64)};
@@ -226,7 +235,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
 bool attn_rows_faster(const KV* kv, int num_seqs, int rows, int num_q_heads, int max_blocks, bool plans) {
     const AttnShape sh = attn_shape(kv, rows, num_q_heads);
     const long long keys = (long long)max_blocks * kv->block_size;
-    if (!sh.full || keys > 64 * kFuseParts) return false;
+    if (!sh.full || keys > 64 * kFuseParts || kv->dtype == GG_DTYPE_INT4) return false;
     const bool wide = kv->head_dim == 128, byte = dtype_bytes(kv->dtype) == 1;
     const double k = (double)keys, heads = (double)num_seqs * rows * num_q_heads;
     const double items = (double)num_seqs * kv->num_kv_heads * sh.groups;

@@ -148,17 +148,28 @@ struct AttnShape {
 // Head_dim 64, or more than 64 query rows per kv head. At head_dim 128 two row tiles and the
 // three bf16 parts of P fit half the register file, at head_dim 64 four do. (A longer group
 // list than the plan's 16-bit head field holds goes to the generic kernel.)
+// 4-bit pools at head_dim 64 or 128 and any row count are tiled the same way (attention_int4.hip), two
+// row tiles at most: `full` stands for row groups of 16 * nt there too.
 inline bool attn_full_supported(const KV* kv, int rows, int num_q_heads) {
     const long long tiles = ((long long)(num_q_heads / kv->num_kv_heads) * rows + 15) / 16;
-    return kv->block_size == 16 && (kv->head_dim == 64 || (kv->head_dim == 128 && tiles > 4)) &&
-           kv->dtype != GG_DTYPE_F32 && kv->dtype != GG_DTYPE_INT4 && kv->num_kv_heads * tiles <= 0x7fff;
+    return kv->block_size == 16 &&
+           (kv->head_dim == 64 || (kv->head_dim == 128 && (tiles > 4 || kv->dtype == GG_DTYPE_INT4))) &&
+           kv->dtype != GG_DTYPE_F32 && kv->num_kv_heads * tiles <= 0x7fff;
 }
 inline AttnShape attn_shape(const KV* kv, int rows, int num_q_heads) {
     const int tiles = (num_q_heads / kv->num_kv_heads * rows + 15) / 16;
     if (!attn_full_supported(kv, rows, num_q_heads)) return {false, tiles, 1};
-    const int most = kv->head_dim == 64 ? 4 : 2;
+    const int most = kv->head_dim == 64 && kv->dtype != GG_DTYPE_INT4 ? 4 : 2;
     const int groups = (tiles + most - 1) / most;
     return {true, (tiles + groups - 1) / groups, groups};
+}
+
+// The two for a pool: 4-bit ones take 64-token chunks, two workgroups per CU.
+inline int attn_kv_chunk_tokens(const KV* kv, int nt) {
+    return kv->dtype == GG_DTYPE_INT4 ? 64 : attn_chunk_tokens((int)dtype_bytes(kv->dtype), nt);
+}
+inline int attn_kv_occupancy(const KV* kv, int nt) {
+    return kv->dtype == GG_DTYPE_INT4 ? 2 : attn_occupancy((int)dtype_bytes(kv->dtype), nt, kv->head_dim);
 }
 
 // How one verify_attention call is scheduled.
@@ -215,6 +226,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
 
 gg_status_t launch_attn_mfma(const AttnArgs& a, const KVView& kv, hipStream_t s);
 gg_status_t launch_attn_full(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s);
+gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s);
 gg_status_t launch_append_from_tables(const AttnArgs& a, const KVView& kv, hipStream_t s);
 
 #ifdef __HIPCC__

@@ -1,0 +1,563 @@
+// attention_int4.hip — the MFMA attention kernel of 4-bit pools: head_dim 64 or 128, 16-token blocks.
+//
+// A 256-thread workgroup takes one piece of an item (a sequence, a kv head and up to 16 * NT of its
+// G * R query rows): the plan's pieces as in attention_mfma.h, or the whole item where nothing would
+// be cut. Its four waves stream disjoint chunks of 64 tokens (four blocks) and merge at the end.
+// Lane = 16 * g4 + c16.
+//
+// Mathematics. A token's key is s_k (n - z_k) and its value s_v (m - z_v), n and m whole 0..15.
+//   score     = s_k (sum q n - z_k sum q): the products run over the codes alone. The zero point is
+//               one more step of the contraction: operand (z, z) against (-sum q) in two f16 parts.
+//   P.V       = sum p s_v m - sum p s_v z_v: p s_v is the A operand, the codes and, as one more
+//               column tile, the zero points are B operands; the difference is taken at the end.
+// Codes go into the f16 operands without a conversion: the bits 0..15 (or 16 times that, the upper
+// half of a byte left in place) are the f16 subnormals n * 2^-24 (n * 2^-20), which
+// v_mfma_f32_16x16x32_f16 takes exactly. Eight codes cost one shift and four ands (an or with 0x6400
+// and a subtraction per pair would make it nine), the power of two goes into the score's multiplier,
+// and the 16 of every other operand pair into the queries (K) or the column tile (V).
+//   S^T = K . Q^T : lane holds token 4 * (c16 / 4) + ... of its S tile as the A row, dims of lane group
+//               g4 as k. A K row is head_dim / 2 bytes, its lane group's run one 16- or 8-byte load.
+//               The result gives lane (g4, c16) row c16 and the 16 tokens of block g4.
+//   O += P . V  : those 16 tokens are the A operand as they are; the V tile [D/2][16] gives a lane 16
+//               tokens of dims i and i + D/2 in one 16-byte load, two column tiles.
+// Each token's scales and zero points are one word; a wave puts the chunk's 64 words through LDS (one
+// load a lane instead of sixteen).
+//
+// p s_v is held in f16 in units of B 2^-15, B a power of two at or above every s_v the wave has seen
+// (O is rescaled when it grows). Values whose scales lie up to 2^12 apart keep 11 bits down to
+// p = 2^-17 that way; a piece whose scales lie further apart is computed row by row in fp32. Each
+// query row has a power of two of its own (its largest |q| in [2^7, 2^8)), so rows do not touch.
+// PREC (fp32 queries or outputs): queries and p s_v in two f16 parts each, 22 bits, and the zero points
+// are taken from the codes in the operands (f16, exact). Summed apart, codes and zero points leave a
+// rounding of 2^-20 of the row's range, which f16 probabilities hide and fp32 results would show;
+// subtracting is 64 + 16 * 4 instructions more a chunk.
+#include "attention_mfma.h"
+
+namespace gg {
+namespace {
+
+constexpr int kI4Tok = 64;                // tokens of a chunk
+constexpr float kI4Spread = 4096.f;       // ratio of value scales that f16 probabilities take
+constexpr uint32_t kLoNib = 0x000f000fu, kHiNib = 0x00f000f0u;
+
+// Eight codes of a K dword as an MFMA operand: (n0, n4), 16 (n1, n5), (n2, n6), 16 (n3, n7).
+__device__ __forceinline__ uint4 k_operand8(uint32_t w) {
+    const uint32_t u = w >> 8;
+    return make_uint4(w & kLoNib, w & kHiNib, u & kLoNib, u & kHiNib);
+}
+
+__device__ __forceinline__ uint32_t pk_sub_f16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) - __builtin_bit_cast(f16x2, b));
+}
+// An operand's codes less their zero points: z for the first and third pair, 16 z for the others.
+__device__ __forceinline__ uint4 less_zero(uint4 v, uint32_t z0, uint32_t z1, uint32_t z2, uint32_t z3) {
+    return make_uint4(pk_sub_f16(v.x, z0), pk_sub_f16(v.y, z1), pk_sub_f16(v.z, z2), pk_sub_f16(v.w, z3));
+}
+
+__device__ __forceinline__ uint32_t f16_pair(float a, float b) { return cvt_pk_f16(a, b); }
+
+template <int NT, int HD, bool PREC>
+struct Int4Shared {
+    static constexpr int kMM = HD / 32, kParts = PREC ? 2 : 1;
+    uint4 q[kParts][NT][kMM][64];   // B operands of S
+    uint32_t qz[NT * 16];           // -sum q of a row, two f16 parts
+    float qmul[NT * 16];            // the row's score multiplier, log2 domain
+    uint32_t words[kWaves][kI4Tok];
+    float m[kWaves][NT * 16], l[kWaves][NT * 16];
+    int bad[kWaves];
+    __align__(16) float o[kWaves][16][HD + 4];
+};
+
+// Row `row` of the piece by the per-row kernel's steps, for pieces whose value scales are too far apart.
+template <int HD>
+__device__ __forceinline__ void int4_piece_by_rows(const AttnArgs& a, const KVView& kv, const PieceDesc& d, int rows,
+                                                   int rec_rows, float* s_row) {
+    constexpr int kDC = HD / 64;
+    const int G = a.num_q_heads / kv.Hkv, lane = threadIdx.x & 63;
+    float* s_q = s_row;
+    float* s_p = s_row + HD;
+    size_t* s_vrow = (size_t*)(s_row + HD + 64);
+    for (int r = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); r < rows; r += kWaves) {
+        const int j = (d.row0 + r) / G, g = (d.row0 + r) % G;
+        const size_t obase = (((size_t)d.b * a.rows + j) * a.num_q_heads + (size_t)d.kvh * G + g) * HD;
+        __builtin_amdgcn_wave_barrier();  // (the previous row's reads)
+#pragma unroll
+        for (int c = 0; c < kDC; ++c) s_q[lane + 64 * c] = load_as_f32(a.q, a.q_dtype, obase + lane + 64 * c);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        float acc[kDC], m, l;
+        generic_partition<GG_DTYPE_INT4, kDC, false>(a, kv, d.b, d.kvh, d.t0, min(d.t_end, d.ctx - d.nrows + j + 1), s_q, s_p,
+                                                     s_vrow, acc, m, l);
+        if (d.rec < 0) {
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+            for (int c = 0; c < kDC; ++c) store_from_f32(a.out, a.out_dtype, obase + lane + 64 * c, acc[c] * inv);
+        } else {
+            const size_t q = (size_t)d.rec * rec_rows + r;
+#pragma unroll
+            for (int c = 0; c < kDC; ++c) store_agent(a.ws_acc + q * HD + lane + 64 * c, acc[c]);
+            if (lane == 0) store_agent2(a.ws_ml + q * 2, m, l);
+        }
+    }
+}
+
+// The piece's queries into LDS as MFMA operands, scaled row by row.
+template <int NT, int HD, bool PREC>
+__device__ __forceinline__ void int4_stage_q(const AttnArgs& a, const KVView& kv, const PieceDesc& d, int rows,
+                                             Int4Shared<NT, HD, PREC>& s) {
+    constexpr int kMM = HD / 32, kPer = HD / 8;  // threads of a row: eight dims (one K dword) each
+    const int G = a.num_q_heads / kv.Hkv;
+    const int ch = threadIdx.x % kPer;
+#pragma unroll
+    for (int r = threadIdx.x / kPer; r < 16 * NT; r += 256 / kPer) {
+        float f[8];
+        const bool live = r < rows;
+        const int j = live ? (d.row0 + r) / G : 0, g = live ? (d.row0 + r) % G : 0;
+        const size_t at = (((size_t)d.b * a.rows + j) * a.num_q_heads + (size_t)d.kvh * G + g) * HD + 8 * ch;
+        if (a.q_dtype == GG_DTYPE_F32) {
+            struct __attribute__((packed, aligned(4))) F4 { float4 v; };
+            const float4 x = ((const F4*)((const float*)a.q + at))[0].v, y = ((const F4*)((const float*)a.q + at))[1].v;
+            const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = v[e];
+        } else {
+            struct __attribute__((packed, aligned(2))) U4 { uint4 v; };
+            const uint4 w4 = ((const U4*)((const uint16_t*)a.q + at))->v;
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                f[e] = a.q_dtype == GG_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+            }
+        }
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            f[e] = live ? f[e] : 0.f;
+            mx = fmaxf(mx, fabsf(f[e]));  // (a NaN is passed over)
+        }
+#pragma unroll
+        for (int o = 1; o < kPer; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        int e2 = 8;
+        if (mx > 0.f && mx <= 3.402823466e38f) (void)frexpf(mx, &e2);
+        const int k = e2 - 8;
+        // Two factors: 2^-k alone may overflow.
+        const float s1 = ldexpf(1.f, -(k / 2)), s2 = ldexpf(1.f, -(k - k / 2));
+        // Operand order (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+        float sum = 0.f;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const float down = p & 1 ? 0.0625f : 1.f, up = p & 1 ? 16.f : 1.f;
+            const float x = f[p] * s1 * s2 * down, y = f[p + 4] * s1 * s2 * down;
+            hi[p] = f16_pair(x, y);
+            const float hx = f16_bits_to_f32((uint16_t)hi[p]), hy = f16_bits_to_f32((uint16_t)(hi[p] >> 16));
+            sum += (hx + hy) * up;
+            if constexpr (PREC) {
+                lo[p] = f16_pair(x - hx, y - hy);
+                sum += (f16_bits_to_f32((uint16_t)lo[p]) + f16_bits_to_f32((uint16_t)(lo[p] >> 16))) * up;
+            }
+        }
+        const int slot = 16 * (ch / kMM) + (r & 15);
+        s.q[0][r >> 4][ch % kMM][slot] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if constexpr (PREC) s.q[1][r >> 4][ch % kMM][slot] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+        for (int o = 1; o < kPer; o <<= 1) sum += __shfl_xor(sum, o);
+        if (ch == 0) {
+            const float top = f16_bits_to_f32(f32_to_f16_bits(-sum));
+            s.qz[r] = f16_pair(top, -sum - top);
+            // (The codes are in units of 2^-24. Positive and finite: a hidden score times it stays -inf.)
+            const float mul = ldexpf(a.scale * kLog2e, k + 24);
+            s.qmul[r] = fminf(fmaxf(mul, 0x1p-126f), 3.0e38f);
+        }
+    }
+}
+
+template <int NT, int HD, bool PREC>
+__device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, const PieceDesc& d) {
+    using IO = PieceIO<GG_DTYPE_INT8, kI4Tok, HD>;  // (block ids of 64-token chunks)
+    constexpr int kMM = HD / 32, kVT = HD / 32;     // K operands of a token; 16-byte V loads of a lane
+    constexpr int kParts = PREC ? 2 : 1;
+    constexpr int kKW = HD / 32;                    // dwords of a lane's K run
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g4 = lane >> 4;
+    const int wave_u = __builtin_amdgcn_readfirstlane(wave);
+    const int G = a.num_q_heads / kv.Hkv;
+    const int ctx = d.ctx, nrows = d.nrows;
+    if (nrows <= 0 || nrows > ctx) return;
+    const int rows = min(G * nrows - d.row0, 16 * NT);
+    if (rows <= 0) return;
+    const int first_masked = ctx - nrows;
+    const int nchunks = (d.t_end - d.t0 + kI4Tok - 1) / kI4Tok;
+    __shared__ Int4Shared<NT, HD, PREC> s;
+
+    // The call's own rows in this piece: written first, by the whole workgroup. (Row groups write
+    // the same bytes.)
+    if (a.k_new) {
+        const int j0 = max(0, d.t0 - first_masked), j1 = min(nrows, d.t_end - first_masked);
+        if (j0 < j1) {
+            append_int4_rows(a, kv, d.b, d.kvh, ctx, nrows, j0, j1);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __syncthreads();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        }
+    }
+
+    uint32_t kr[4][kKW];   // K: S tile t, the lane's token of it
+    uint4 vr[kVT];         // V: 16 tokens of dims 16 i + c16 and that plus HD / 2
+    uint32_t wr;           // word of token `lane` of the chunk
+    auto load_k = [&](const LaneBlocks bl) {
+        const int blk = max(bl.k, 0);
+        const uint8_t* p = kv.kc + ((size_t)blk * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)(c16 & 3) * (HD / 2) + 4 * kKW * g4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            if constexpr (kKW == 4) {
+                const uint4 x = *(const uint4*)(p + t * 4 * (HD / 2));
+                kr[t][0] = x.x, kr[t][1] = x.y, kr[t][2] = x.z, kr[t][3] = x.w;
+            } else {
+                const uint2 x = *(const uint2*)(p + t * 4 * (HD / 2));
+                kr[t][0] = x.x, kr[t][1] = x.y;
+            }
+        }
+        wr = kv.words[((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * kBS + c16];
+    };
+    auto load_v = [&](const LaneBlocks bl) {
+        const uint8_t* p = kv.vc + ((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)c16 * kBS;
+#pragma unroll
+        for (int i = 0; i < kVT; ++i) vr[i] = *(const uint4*)(p + i * 16 * kBS);
+    };
+    const auto fb = IO::first_blocks(a, d);
+    LaneBlocks bl_cur = IO::lane_blocks(kv, fb.r0, d.t_end), bl_next = IO::lane_blocks(kv, fb.r1, d.t_end);
+    load_k(bl_cur);
+    load_v(bl_cur);
+
+    int4_stage_q<NT, HD, PREC>(a, kv, d, rows, s);
+    __syncthreads();
+
+    uint32_t qz[NT];
+    float qmul[NT];
+    int row_pos[NT];  // last key that row c16 sees
+#pragma unroll
+    for (int rt = 0; rt < NT; ++rt) {
+        const int r = rt * 16 + c16;
+        qz[rt] = g4 == 0 ? s.qz[r] : 0u;  // k = 0, 1 of the contraction: lane group 0
+        qmul[rt] = s.qmul[r];
+        row_pos[rt] = r < rows ? first_masked + (d.row0 + r) / G : ctx - 1;
+    }
+
+    f32x4 o[NT][2 * kVT], oz[NT];
+    float m_run[NT], l_run[NT];
+#pragma unroll
+    for (int rt = 0; rt < NT; ++rt) {
+        m_run[rt] = -1e30f;
+        l_run[rt] = 0.f;
+        oz[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < 2 * kVT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float bound = 0.f, vnorm = 0.f;   // B, and 2^15 / B (wave-uniform)
+    float vs_min = 3.0e38f;           // smallest value scale of the lane's tokens
+
+    for (int ch = wave_u; ch < nchunks; ch += kWaves) {
+        const int tc = d.t0 + ch * kI4Tok;
+        const int tlane = tc + 16 * g4;  // first token of the lane's block
+        const bool missing = bl_cur.v < 0;
+
+        // The chunk's words to LDS (this wave's own slots: its LDS operations run in order).
+        {
+            __builtin_amdgcn_wave_barrier();
+            s.words[wave][lane] = wr;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            // Value scales past B: B grows, and what has been summed shrinks with it.
+            float vs = int4_v_scale(wr);
+            vs = !missing && tlane + c16 < ctx ? vs : 0.f;
+            vs_min = vs > 0.f ? fminf(vs_min, vs) : vs_min;
+            if (__builtin_expect(__any(vs > bound), 0)) {
+                const float top = wave_max(vs);
+                const float grown = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
+                const float f = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(bound / grown)));
+                bound = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(grown)));
+                vnorm = 32768.f / bound;
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt) {
+                    oz[rt] *= f;
+#pragma unroll
+                    for (int t = 0; t < 2 * kVT; ++t) o[rt][t] *= f;
+                }
+            }
+        }
+
+        // ---- S^T = K . Q^T ----
+        // (The Q index is opaque, so that the LDS reads stay in the loop.)
+        int qlane;
+        asm("" : "=v"(qlane) : "0"(lane), "s"(ch));
+        f32x4 sacc[NT][4];
+#pragma unroll
+        for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) sacc[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t kz[4];  // zero point of the lane's token of S tile t, a pair
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint32_t z = s.words[wave][16 * (c16 >> 2) + 4 * t + (c16 & 3)] & 15u;
+            kz[t] = z | (z << 16);
+        }
+#pragma unroll
+        for (int mm = 0; mm < kMM; ++mm) {
+            uint4 qop[kParts][NT];
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt) qop[p][rt] = s.q[p][rt][mm][qlane];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                uint4 kop = k_operand8(kr[t][mm]);
+                if constexpr (PREC) kop = less_zero(kop, kz[t], kz[t] << 4, kz[t], kz[t] << 4);
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) sacc[rt][t] = mfma(kop, qop[p][rt], sacc[rt][t], false);
+            }
+        }
+        if constexpr (!PREC) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt)
+                    sacc[rt][t] = mfma(make_uint4(kz[t], 0u, 0u, 0u), make_uint4(qz[rt], 0u, 0u, 0u), sacc[rt][t], false);
+        }
+        uint32_t w[16];  // words of the lane's block
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const uint4 x = *(const uint4*)&s.words[wave][16 * g4 + 4 * t];
+            w[4 * t] = x.x, w[4 * t + 1] = x.y, w[4 * t + 2] = x.z, w[4 * t + 3] = x.w;
+        }
+        load_k(bl_next);
+
+        // ---- online softmax ----
+        const bool need_mask = tc + kI4Tok - 1 >= first_masked || __any(missing);
+        uint32_t pop[NT][kParts][8];
+        float ks[16], vs[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            ks[i] = int4_k_scale(w[i]);
+            vs[i] = int4_v_scale(w[i]) * vnorm;
+        }
+        if (__builtin_expect(need_mask, 0)) {  // (stale words may hold any scale: 0 times it must be 0)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) vs[i] = !missing && tlane + i < ctx ? vs[i] : 0.f;
+        }
+#pragma unroll
+        for (int rt = 0; rt < NT; ++rt) {
+            float sc[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = sacc[rt][i >> 2][i & 3] * ks[i];
+            if (__builtin_expect(need_mask, 0)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sc[i] = !missing && tlane + i <= row_pos[rt] ? sc[i] : -INFINITY;
+            }
+            float cmax = sc[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) cmax = fmaxf(cmax, sc[i]);
+            cmax = max_over_rows(cmax * qmul[rt]);
+            const float m_new = fmaxf(m_run[rt], cmax);
+            const float alpha = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+            m_run[rt] = m_new;
+            float psum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qmul[rt], -m_new));
+                psum += sc[i];
+                sc[i] *= vs[i];
+            }
+            l_run[rt] = l_run[rt] * alpha + psum;
+            if (__any(alpha != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float al = __shfl(alpha, 4 * g4 + i);
+                    oz[rt][i] *= al;
+#pragma unroll
+                    for (int t = 0; t < 2 * kVT; ++t) o[rt][t][i] *= al;
+                }
+            }
+            // Operand order of a V dword: tokens (0, 2), (1, 3).
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x = sc[4 * q + e], y = sc[4 * q + e + 2];
+                    const uint32_t h = f16_pair(x, y);
+                    pop[rt][0][2 * q + e] = h;
+                    if constexpr (PREC)
+                        pop[rt][1][2 * q + e] =
+                            f16_pair(x - f16_bits_to_f32((uint16_t)h), y - f16_bits_to_f32((uint16_t)(h >> 16)));
+                }
+        }
+        const typename IO::RawBlocks raw_after = IO::fetch_blocks(a, d.b, d.t0, ch + 2 * kWaves);
+
+        // ---- O += P . V, the zero points as one more column tile ----
+        uint32_t vz[2][4];  // zero points in operand order
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = 8 * half + 4 * (i >> 1) + (i & 1);  // tokens t, t + 2
+                vz[half][i] = __builtin_amdgcn_perm(w[t + 2], w[t], 0x07060302u) & kLoNib;
+            }
+            if constexpr (!PREC) {
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt) {
+                    const uint32_t* q = pop[rt][0] + 4 * half;
+                    oz[rt] = mfma(make_uint4(q[0], q[1], q[2], q[3]),
+                                  make_uint4(vz[half][0], vz[half][1], vz[half][2], vz[half][3]), oz[rt], false);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kVT; ++i) {
+            const uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t x = v[2 * half], y = v[2 * half + 1], x8 = x >> 8, y8 = y >> 8;
+                uint4 lo = make_uint4(x & kLoNib, x8 & kLoNib, y & kLoNib, y8 & kLoNib);
+                uint4 hi = make_uint4(x & kHiNib, x8 & kHiNib, y & kHiNib, y8 & kHiNib);
+                if constexpr (PREC) {
+                    const uint32_t* z = vz[half];
+                    lo = less_zero(lo, z[0], z[1], z[2], z[3]);
+                    hi = less_zero(hi, z[0] << 4, z[1] << 4, z[2] << 4, z[3] << 4);
+                }
+#pragma unroll
+                for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p) {
+                        const uint32_t* q = pop[rt][p] + 4 * half;
+                        const uint4 pa = make_uint4(q[0], q[1], q[2], q[3]);
+                        o[rt][i] = mfma(pa, lo, o[rt][i], false);
+                        o[rt][i + kVT] = mfma(pa, hi, o[rt][i + kVT], false);
+                    }
+            }
+        }
+        load_v(bl_next);
+        bl_cur = bl_next;
+        bl_next = IO::lane_blocks(kv, raw_after, d.t_end);
+    }
+
+    // ---- merge the four waves ----
+#pragma unroll
+    for (int rt = 0; rt < NT; ++rt) {
+        float lt = l_run[rt];
+        lt += __shfl_xor(lt, 16);
+        lt += __shfl_xor(lt, 32);
+        if (g4 == 0) {
+            s.m[wave][rt * 16 + c16] = m_run[rt];
+            s.l[wave][rt * 16 + c16] = lt;
+        }
+    }
+    const float lowest = wave_min(vs_min);
+    if (lane == 0) s.bad[wave] = bound > kI4Spread * lowest;
+    __syncthreads();
+    if (__builtin_expect(s.bad[0] | s.bad[1] | s.bad[2] | s.bad[3], 0)) {
+        int4_piece_by_rows<HD>(a, kv, d, rows, 16 * NT, &s.o[wave][0][0]);
+        return;
+    }
+    const float unit = bound * 512.f;  // codes in 2^-24, p s_v in B 2^-15
+    for (int rt = 0; rt < NT; ++rt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rr = 4 * g4 + i, r = rt * 16 + rr;
+            float mx = s.m[0][r];
+#pragma unroll
+            for (int u = 1; u < kWaves; ++u) mx = fmaxf(mx, s.m[u][r]);
+            const float f = __builtin_amdgcn_exp2f(s.m[wave][r] - mx) * unit;
+#pragma unroll
+            for (int t = 0; t < kVT; ++t) {
+                s.o[wave][rr][t * 16 + c16] = (o[rt][t][i] - oz[rt][i]) * f;
+                s.o[wave][rr][HD / 2 + t * 16 + c16] = (__builtin_fmaf(o[rt][t + kVT][i], 0.0625f, -oz[rt][i])) * f;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = threadIdx.x; e < 16 * (HD / 4); e += 256) {
+            const int rr = e / (HD / 4), dim = 4 * (e % (HD / 4)), r = rt * 16 + rr;
+            if (r >= rows) continue;
+            float mx = s.m[0][r];
+#pragma unroll
+            for (int u = 1; u < kWaves; ++u) mx = fmaxf(mx, s.m[u][r]);
+            float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < kWaves; ++u) {
+                L += s.l[u][r] * __builtin_amdgcn_exp2f(s.m[u][r] - mx);
+                const float4 v = *(const float4*)&s.o[u][rr][dim];
+                acc[0] += v.x;
+                acc[1] += v.y;
+                acc[2] += v.z;
+                acc[3] += v.w;
+            }
+            if (d.rec < 0) {
+                const int j = (d.row0 + r) / G, h = d.kvh * G + (d.row0 + r) % G;
+                float val[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) val[k] = L == 0.f ? 0.f : acc[k] / L;  // (a NaN stays one)
+                store4_from_f32(a.out, a.out_dtype, (((size_t)d.b * a.rows + j) * a.num_q_heads + h) * HD + dim, val);
+            } else {
+                const size_t p = (size_t)d.rec * (16 * NT) + r;
+                store_agent2(a.ws_acc + p * HD + dim, acc[0], acc[1]);
+                store_agent2(a.ws_acc + p * HD + dim + 2, acc[2], acc[3]);
+                if (dim == 0) store_agent2(a.ws_ml + p * 2, mx > -1e29f ? mx * kLn2 : -1e30f, L);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// PLANNED: workgroup p runs the plan's piece p, and the last piece of a split item merges it. Else
+// workgroup (sequence, head) runs the whole item: calls too narrow to cut, and batches that the
+// plan does not rank.
+template <int NT, int HD, bool PREC, bool PLANNED>
+__global__ void __launch_bounds__(256, 2) attn_int4_kernel(AttnArgs a, KVView kv) {
+    const int heads = kv.Hkv * a.row_groups;
+    if constexpr (PLANNED) {
+        const int p = blockIdx.x;
+        const int4 e = ((const int4*)lpt_table(a.plan))[2 * p], f = ((const int4*)lpt_table(a.plan))[2 * p + 1];
+        if (e.x < 0) return;  // past the last piece
+        const int h = e.y & 0xffff, np = e.y >> 16, row0 = h / kv.Hkv * (16 * NT);
+        const PieceDesc d{e.x, h % kv.Hkv, e.z, e.w, -1, np > 1 ? f.z + f.w * heads : -1, row0, f.x, f.y};
+        int4_piece<NT, HD, PREC>(a, kv, d);
+        if (np > 1 && a.num_q_heads / kv.Hkv * d.nrows > row0) lpt_merge_if_last<HD>(a, kv.Hkv, heads, d, h, np, f.z, 16 * NT);
+    } else {
+        const int h = blockIdx.x % heads, b = blockIdx.x / heads;
+        const int ctx = seq_keys(a, b, kBS), nrows = seq_rows(a, b);
+        int4_piece<NT, HD, PREC>(a, kv, PieceDesc{b, h % kv.Hkv, 0, ctx, -1, -1, h / kv.Hkv * (16 * NT), ctx, nrows});
+    }
+}
+
+template <int NT, int HD, bool PREC>
+void launch_one(const AttnArgs& a, const KVView& kv, hipStream_t s) {
+    if (a.sched == ATTN_SCHED_LPT)
+        attn_int4_kernel<NT, HD, PREC, true><<<lpt_pieces(a.sk_grid, a.num_seqs, kv.Hkv * a.row_groups), 256, 0, s>>>(a, kv);
+    else
+        attn_int4_kernel<NT, HD, PREC, false><<<a.num_seqs * kv.Hkv * a.row_groups, 256, 0, s>>>(a, kv);
+}
+
+template <int NT, int HD>
+void launch_prec(const AttnArgs& a, const KVView& kv, hipStream_t s) {
+    if (a.q_dtype == GG_DTYPE_F32 || a.out_dtype == GG_DTYPE_F32) launch_one<NT, HD, true>(a, kv, s);
+    else launch_one<NT, HD, false>(a, kv, s);
+}
+
+}  // namespace
+
+gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s) {
+    if (kv.D == 128) {
+        if (sh.nt == 1) launch_prec<1, 128>(a, kv, s);
+        else launch_prec<2, 128>(a, kv, s);
+    } else {
+        if (sh.nt == 1) launch_prec<1, 64>(a, kv, s);
+        else launch_prec<2, 64>(a, kv, s);
+    }
+    return check_hip(hipGetLastError(), "verify_attention launch");
+}
+
+}  // namespace gg

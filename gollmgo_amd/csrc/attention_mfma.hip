@@ -385,11 +385,12 @@ gg_status_t launch_attn_mfma(const AttnArgs& a, const KVView& kv, hipStream_t s)
     const AttnShape sh = attn_shape(a.kv, a.rows, a.num_q_heads);
     const int G = a.num_q_heads / kv.Hkv;
     const int nt = sh.nt;
-    const int tok = attn_chunk_tokens(dtype_bytes(kv.dt), nt);
+    const int tok = attn_kv_chunk_tokens(a.kv, nt);
     if (a.sched == ATTN_SCHED_LPT && !a.plan_ready) {
         const gg_status_t st = launch_attn_plan(a, s);
         if (st != GG_OK) return st;
     }
+    if (kv.dt == GG_DTYPE_INT4) return launch_attn_int4(a, kv, sh, s);
     if (sh.full) return launch_attn_full(a, kv, sh, s);
     gg_status_t st;
     switch (kv.dt) {
@@ -413,7 +414,7 @@ gg_status_t launch_attn_plan(const AttnArgs& a, hipStream_t s) {
     const int Hkv = kv->num_kv_heads;
     const AttnShape sh = attn_shape(kv, a.rows, a.num_q_heads);
     const int heads = Hkv * sh.groups;
-    const int tok = attn_chunk_tokens(dtype_bytes(kv->dtype), sh.nt);
+    const int tok = attn_kv_chunk_tokens(kv, sh.nt);
     const int pieces = lpt_pieces(a.sk_grid, a.num_seqs, heads);
     const int tok_log2 = tok == 64 ? 6 : 5;
     if (a.num_seqs <= 256) attn_lpt_plan_kernel<256><<<1, 256, 0, s>>>(a, heads, tok_log2, a.sk_grid, pieces);
@@ -423,11 +424,14 @@ gg_status_t launch_attn_plan(const AttnArgs& a, hipStream_t s) {
 
 int attn_slots(const KV* kv, int rows, int num_q_heads) {
     // One resident wave of workgroups: each CU holds attn_occupancy of them.
-    return device_cu_count() * attn_occupancy((int)dtype_bytes(kv->dtype), attn_shape(kv, rows, num_q_heads).nt, kv->head_dim);
+    return device_cu_count() * attn_kv_occupancy(kv, attn_shape(kv, rows, num_q_heads).nt);
 }
 
 size_t attn_record_workspace_bytes(const KV* kv, int sched, int num_seqs, int rows, int num_q_heads, int max_blocks,
                                    size_t* ml_elems, size_t* acc_elems) {
+    if (ml_elems) *ml_elems = 0;
+    if (acc_elems) *acc_elems = 0;
+    if (sched == ATTN_SCHED_ITEMS) return 0;
     const AttnShape sh = attn_shape(kv, rows, num_q_heads);
     const int slots = attn_slots(kv, rows, num_q_heads);
     const int heads = kv->num_kv_heads * sh.groups;
@@ -446,6 +450,7 @@ size_t attn_record_workspace_bytes(const KV* kv, int sched, int num_seqs, int ro
     // The size asked for is never below a record per slot and item and its plan, or, for the
     // shapes the per-row kernel also serves, that kernel's: callers size buffers by it, and
     // gg_verify_attention_noalloc takes the calls that fit its fixed array by this measure.
+    if (kv->dtype == GG_DTYPE_INT4) return need;
     const size_t asked = sh.full ? attn_workspace_bytes(kv, num_seqs, rows, num_q_heads, max_blocks,
                                                         attn_generic_partition(kv, num_seqs, rows, num_q_heads, max_blocks))
                                  : bytes((size_t)slots + items, gr, 16 + 4 * ((size_t)slots + items) + 2 * (size_t)num_seqs + items);

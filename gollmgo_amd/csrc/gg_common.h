@@ -108,8 +108,9 @@ struct AttnArgs {
     const void* v_new;
     gg_dtype_t new_dtype;
 };
-// Attention schedules on the MFMA path (the generic path always uses the grid).
-enum { ATTN_SCHED_GRID = 0, ATTN_SCHED_STREAMK = 1, ATTN_SCHED_LPT = 2 };
+// Attention schedules on the MFMA path (the generic path always uses the grid). ITEMS: a workgroup
+// per item of a 4-bit pool, no plan and no workspace.
+enum { ATTN_SCHED_GRID = 0, ATTN_SCHED_STREAMK = 1, ATTN_SCHED_LPT = 2, ATTN_SCHED_ITEMS = 3 };
 
 // Stream-K and LPT: resident workgroup slots for a shape on the current device, and the
 // workspace of a schedule: partial records (LPT: one per piece of a split item; stream-K: grid

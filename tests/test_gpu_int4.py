@@ -280,11 +280,11 @@ def check_attention(gv, kv, tables, rng, ctx, rows, R, hq, qdt="bf16", odt="bf16
     cd = torch.from_numpy(np.asarray(ctx, np.int32)).cuda()
     rd = torch.from_numpy(np.asarray(rows, np.int32)).cuda() if rows is not None else None
     kv.attention(layer, qd, out, cd, torch.from_numpy(tables).cuda(), scale, row_counts=rd, partition_tokens=partition, **kw)
-    K, V = ref.pool_values(kv, layer)
-    want, mag = ref.attention(qf.astype(np.float64), K, V, ctx, rows if rows is not None else [R] * B, tables, scale,
-                              np.full(q.shape, 11.0))
+    K, V, k_span, v_span = ref.pool_values(kv, layer, spans=True)
+    want, mag, reach, least = ref.attention(qf.astype(np.float64), K, V, ctx, rows if rows is not None else [R] * B, tables, scale,
+                                            np.full(q.shape, 11.0), v_span)
     got = out.double().cpu().numpy()
-    tol = ref.attention_tolerance(qf.astype(np.float64), K, V, scale, want, mag, qdt, odt)
+    tol = ref.attention_tolerance(qf.astype(np.float64), K, k_span, scale, want, mag, reach, least, qdt, odt)
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5], tol[bad][:5])
     return got
