@@ -41,6 +41,11 @@ class ScaleMode(enum.IntEnum):
     PER_TOKEN = 3
 
 
+class RopeStyle(enum.IntEnum):
+    HALVES = 0
+    PAIRS = 1
+
+
 class GGError(RuntimeError):
     def __init__(self, status: int, where: str, msg: str):
         super().__init__(f"{where}: status {Status(status).name}: {msg}")
@@ -51,6 +56,7 @@ _vp = C.c_void_p
 _i = C.c_int
 _f = C.c_float
 _sz = C.c_size_t
+_ll = C.c_longlong
 _i32p = C.POINTER(C.c_int32)
 
 # name -> (restype, argtypes)
@@ -68,6 +74,9 @@ SIGNATURES = {
     "gg_kv_layer_bytes": (_sz, [_vp]),
     "gg_kv_set_head_scales": (_i, [_vp, _i, C.POINTER(_f), C.POINTER(_f)]),
     "gg_kv_append": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
+    "gg_qk_norm_rope": (_i, [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "gg_qk_norm_rope_append": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _i, _i,
+                                    _vp, _vp, _vp]),
     "gg_kv_read": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
     "gg_kv_snapshot_bytes": (_sz, [_vp, _i]),
     "gg_kv_snapshot": (_i, [_vp, _vp, _i, _vp, _sz, _vp, _vp]),

@@ -251,6 +251,105 @@ GG_API gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void
     return launch_kv_append(kv, layer, k, v, src_dtype, slot_mapping, n_rows, (hipStream_t)stream);
 }
 
+// ---------------------------------------------------------------- norm and rotation
+
+static gg_status_t rope_args(RopeArgs& a, const char* who, const void* q, long long q_stride, const void* k, long long k_stride,
+                             gg_dtype_t dtype, int n_rows, int num_q_heads, int num_kv_heads, int head_dim,
+                             const void* q_weight, const void* k_weight, float eps, const int32_t* positions, int num_axes,
+                             const uint8_t* pair_axis, const float* inv_freq, int num_pairs, gg_rope_style_t style,
+                             void* q_out) {
+    const std::string w = who;
+#define GG_CHECK_ROPE(cond, msg) \
+    do {                         \
+        if (!(cond)) return fail(GG_ERR_INVALID, w + ": " + (msg)); \
+    } while (0)
+    GG_CHECK_ROPE(is_float_io(dtype), "dtype must be F32/F16/BF16");
+    GG_CHECK_ROPE(n_rows >= 0 && n_rows <= (1 << 24), "n_rows out of range");
+    GG_CHECK_ROPE(num_q_heads >= 0 && num_kv_heads >= 0 && num_q_heads + (long long)num_kv_heads > 0 &&
+                      num_q_heads + (long long)num_kv_heads <= (1 << 16),
+                  "bad head count");
+    GG_CHECK_ROPE(head_dim > 0 && head_dim <= 1024, "head_dim must be 1..1024");
+    GG_CHECK_ROPE(num_pairs >= 0 && num_pairs <= kRopeMaxPairs && 2 * num_pairs <= head_dim,
+                  "num_pairs must be 0..512, two dims each within head_dim");
+    GG_CHECK_ROPE(num_axes >= 1 && num_axes <= kRopeMaxAxes, "num_axes must be 1..8");
+    GG_CHECK_ROPE(style == GG_ROPE_HALVES || style == GG_ROPE_PAIRS, "unknown style");
+    GG_CHECK_ROPE(std::isfinite(eps) && eps >= 0.f, "eps must be finite and >= 0");
+    GG_CHECK_ROPE(q_stride >= (long long)num_q_heads * head_dim && k_stride >= (long long)num_kv_heads * head_dim,
+                  "rows overlap (stride below heads * head_dim)");
+    if (n_rows > 0) {
+        GG_CHECK_ROPE(num_q_heads == 0 || (q && q_out), "NULL buffer");
+        GG_CHECK_ROPE(num_kv_heads == 0 || k, "NULL buffer");
+        GG_CHECK_ROPE(num_pairs == 0 || (positions && inv_freq), "NULL buffer");
+    }
+    for (int j = 0; j < num_pairs; ++j) {
+        const int ax = pair_axis ? pair_axis[j] : 0;
+        GG_CHECK_ROPE(ax < num_axes, "pair_axis names an axis that positions does not have");
+        a.axis[j / 8] |= (uint32_t)ax << (4 * (j % 8));
+    }
+#undef GG_CHECK_ROPE
+    a.q = q;
+    a.k = k;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.dt = dtype;
+    a.n = n_rows;
+    a.Hq = num_q_heads;
+    a.Hkv = num_kv_heads;
+    a.D = head_dim;
+    a.q_weight = q_weight;
+    a.k_weight = k_weight;
+    a.eps = eps;
+    a.positions = positions;
+    a.inv_freq = inv_freq;
+    a.pairs = num_pairs;
+    a.style = style;
+    a.q_out = q_out;
+    return GG_OK;
+}
+
+GG_API gg_status_t gg_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride,
+                                   gg_dtype_t dtype, int n_rows, int num_q_heads, int num_kv_heads, int head_dim,
+                                   const void* q_weight, const void* k_weight, float eps, const int32_t* positions,
+                                   int num_axes, const uint8_t* pair_axis, const float* inv_freq, int num_pairs,
+                                   gg_rope_style_t style, void* q_out, void* k_out, void* stream) {
+    clear_error();
+    RopeArgs a{};
+    const gg_status_t st = rope_args(a, "gg_qk_norm_rope", q, q_stride, k, k_stride, dtype, n_rows, num_q_heads, num_kv_heads,
+                                     head_dim, q_weight, k_weight, eps, positions, num_axes, pair_axis, inv_freq, num_pairs,
+                                     style, q_out);
+    if (st != GG_OK) return st;
+    if (n_rows == 0) return GG_OK;
+    GG_CHECK_ARG(num_kv_heads == 0 || k_out, "gg_qk_norm_rope: NULL buffer");
+    a.k_out = k_out;
+    return launch_qk_norm_rope(a, nullptr, 0, (hipStream_t)stream);
+}
+
+GG_API gg_status_t gg_qk_norm_rope_append(gg_kv_t kv, int layer, const void* q, long long q_stride, const void* k,
+                                          long long k_stride, const void* v, long long v_stride, gg_dtype_t dtype,
+                                          int n_rows, int num_q_heads, const void* q_weight, const void* k_weight,
+                                          float eps, const int32_t* positions, int num_axes, const uint8_t* pair_axis,
+                                          const float* inv_freq, int num_pairs, gg_rope_style_t style, void* q_out,
+                                          const int32_t* slot_mapping, void* stream) {
+    clear_error();
+    GG_CHECK_ARG(kv != nullptr, "gg_qk_norm_rope_append: kv is NULL");
+    GG_CHECK_ARG(layer >= 0 && layer < kv->num_layers, "gg_qk_norm_rope_append: layer out of range");
+    GG_CHECK_ARG(kv->scale_mode != GG_SCALE_PER_BLOCK,
+                 "gg_qk_norm_rope_append: PER_BLOCK pools are not taken (gg_qk_norm_rope, then gg_kv_append)");
+    RopeArgs a{};
+    const gg_status_t st = rope_args(a, "gg_qk_norm_rope_append", q, q_stride, k, k_stride, dtype, n_rows, num_q_heads,
+                                     kv->num_kv_heads, kv->head_dim, q_weight, k_weight, eps, positions, num_axes, pair_axis,
+                                     inv_freq, num_pairs, style, q_out);
+    if (st != GG_OK) return st;
+    GG_CHECK_ARG(v_stride >= (long long)kv->num_kv_heads * kv->head_dim,
+                 "gg_qk_norm_rope_append: rows overlap (stride below heads * head_dim)");
+    if (n_rows == 0) return GG_OK;
+    GG_CHECK_ARG(v && slot_mapping, "gg_qk_norm_rope_append: NULL buffer");
+    a.v = v;
+    a.v_stride = v_stride;
+    a.slots = slot_mapping;
+    return launch_qk_norm_rope(a, kv, layer, (hipStream_t)stream);
+}
+
 GG_API gg_status_t gg_kv_read(gg_kv_t kv, int layer, void* k_out, void* v_out, gg_dtype_t out_dtype,
                               const int32_t* slot_mapping, int n_rows, void* stream) {
     clear_error();

@@ -74,6 +74,31 @@ gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* 
 gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype_t dst, const int32_t* slots, int n_rows,
                            hipStream_t s);
 
+// Norm and rotation of query and key rows (qk_norm_rope.hip).
+constexpr int kRopeMaxAxes = 8;
+constexpr int kRopeMaxPairs = 512;
+struct RopeArgs {
+    const void* q;
+    const void* k;
+    const void* v;               // rows for the pool, or null
+    long long q_stride, k_stride, v_stride;
+    gg_dtype_t dt;
+    int n, Hq, Hkv, D;
+    const void* q_weight;        // null: no norm
+    const void* k_weight;
+    float eps;
+    const int32_t* positions;    // [axes][n]
+    const float* inv_freq;
+    int pairs;                   // P
+    int style;                   // gg_rope_style_t
+    void* q_out;
+    void* k_out;                 // null: keys go to the pool
+    const int32_t* slots;
+    // Pair j's axis in bits 4 * (j % 8) of word j / 8 (axes below 8 fit).
+    uint32_t axis[kRopeMaxPairs / 8];
+};
+gg_status_t launch_qk_norm_rope(const RopeArgs& a, KV* kv, int layer, hipStream_t s);
+
 struct AttnArgs {
     const KV* kv;
     int layer;

@@ -7,6 +7,8 @@ of libgg_verify.so. Names follow the reference's domain:
   KVCache            ~ CUDAKVCache (internal/backend/cuda/kvcache_bridge.go:16-91)
   KVCache.append     ~ CUDAKVCache.Write / gollmgo_kvcache_write
   KVCache.read       (none) rows of a pool as numbers
+  qk_norm_rope       ~ rope_f16 (kernels/gollmgo_ops.cu:88-128), with per-head norms
+  KVCache.norm_rope_append  the same with keys and values written to the cache
   KVCache.attention  ~ gollmgo_kvcache_attention, for k+1 verify rows per sequence
   accept_greedy      ~ Verify + argmax as emitSpeculative drives them
                        (internal/engine/speculative.go:68-84, serving.go:514-566)
@@ -18,11 +20,11 @@ of libgg_verify.so. Names follow the reference's domain:
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
-from ._lib import DType, ScaleMode, check, lib
+from ._lib import DType, RopeStyle, ScaleMode, check, lib
 
 _TORCH_TO_DT = {torch.float32: DType.F32, torch.float16: DType.F16, torch.bfloat16: DType.BF16}
 
@@ -51,6 +53,81 @@ def _dev(t: torch.Tensor, name: str, dtype=None) -> int:
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, head_dim: Optional[int] = None):
+    """Pointer and row stride of [n_rows, heads, head_dim] rows whose heads are contiguous (a
+    slice of a fused projection, or a whole tensor)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dim() != 3 or (head_dim is not None and t.shape[2] != head_dim):
+        raise ValueError(f"{name} must be [n_rows, heads, head_dim]")
+    n, h, d = t.shape
+    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+        raise ValueError(f"{name}: the heads of a row must be contiguous")
+    return t.data_ptr(), t.stride(0) if n > 1 else h * d
+
+
+def _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style):
+    """The arguments that qk_norm_rope and norm_rope_append share, checked."""
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("q or k is needed")
+    n, _, d = some.shape
+    if k is not None and (k.dim() != 3 or k.shape[0] != n or k.shape[2] != d or k.dtype != some.dtype):
+        raise ValueError("q and k must share rows, head_dim and dtype")
+    pairs = inv_freq.numel()
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    if positions.dim() != 2 or positions.shape[1] != n:
+        raise ValueError("positions must be [n_rows] or [axes, n_rows]")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None and (w.shape != (d,) or w.dtype != some.dtype):
+            raise ValueError(f"{name} must be [head_dim] of the rows' dtype")
+    axis = None
+    if pair_axis is not None:
+        if len(pair_axis) != pairs:
+            raise ValueError("pair_axis must name an axis for each of inv_freq's pairs")
+        if any(not 0 <= int(x) < positions.shape[0] for x in pair_axis):
+            raise ValueError("pair_axis names an axis that positions does not have")
+        axis = (C.c_uint8 * max(pairs, 1))(*[int(x) for x in pair_axis])
+    elif positions.shape[0] != 1:
+        raise ValueError("several position axes need pair_axis")
+    try:
+        st = RopeStyle[style.upper()]
+    except KeyError as e:
+        raise ValueError(f"unknown style {style!r} (halves, pairs)") from e
+    weights = [_dev(w, "weight") if w is not None else None for w in (q_weight, k_weight)]
+    return n, d, pairs, _dev(positions, "positions", torch.int32), positions.shape[0], axis, _dev(
+        inv_freq, "inv_freq", torch.float32), int(st), weights
+
+
+def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 pair_axis: Optional[Sequence[int]] = None, style: str = "halves", q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+    """Norm of each head (where its weight is given) and rotation of the first 2 * len(inv_freq)
+    dims by positions * inv_freq (gg_qk_norm_rope). q [n, Hq, D], k [n, Hkv, D]: rows may be
+    strided (slices of a fused projection); either may be None. positions int32 [n], or
+    [axes, n] with pair_axis naming the axis of each pair. style "halves": dim j with
+    j + pairs; "pairs": 2j with 2j + 1. -> (q_out, k_out), contiguous; q_out may be q itself
+    where that is contiguous."""
+    n, d, pairs, pos, axes, axis, freq, st, (wq, wk) = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style)
+    sides = []
+    for x, o, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if x is None:
+            sides.append((None, 0, 0, None, None))
+            continue
+        ptr, stride = _rows(x, name)
+        if o is None:
+            o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif o.numel() != x.numel() or o.dtype != x.dtype:
+            raise ValueError(f"{name}_out must be like {name}")
+        sides.append((ptr, stride, x.shape[1], _dev(o, f"{name}_out"), o))
+    (qp, qs, hq, qo, q_out), (kp, ks, hk, ko, k_out) = sides
+    check(lib().gg_qk_norm_rope(qp, qs, kp, ks, int(dtype_of(q if q is not None else k)), n, hq, hk, d, wq, wk, float(eps), pos,
+                                axes, axis, freq, pairs, st, qo, ko, _stream(stream)), "gg_qk_norm_rope")
+    return q_out, k_out
 
 
 class _DeviceBuffer:
@@ -155,6 +232,36 @@ class KVCache:
         check(lib().gg_kv_append(self.handle, layer, _dev(k, "k"), _dev(v, "v", k.dtype), int(dtype_of(k)),
                                  _dev(slot_mapping, "slot_mapping", torch.int32), n, _stream(stream)),
               "gg_kv_append")
+
+    def norm_rope_append(self, layer: int, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                         positions: torch.Tensor, inv_freq: torch.Tensor, slot_mapping: torch.Tensor,
+                         q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                         eps: float = 1e-6, pair_axis: Optional[Sequence[int]] = None, style: str = "halves",
+                         q_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
+        """qk_norm_rope with the keys, and the values v [n, Hkv, D] beside them, written to the slots
+        of slot_mapping (gg_qk_norm_rope_append; not for INT8 pools) -> q_out."""
+        n, d, pairs, pos, axes, axis, freq, st, (wq, wk) = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis,
+                                                                 style)
+        if k.shape[1:] != (self.num_kv_heads, self.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
+            raise ValueError("k and v must be [n_rows, num_kv_heads, head_dim] of one dtype")
+        if slot_mapping.numel() != n:
+            raise ValueError("slot_mapping must be [n_rows]")
+        kp, ks = _rows(k, "k")
+        vp, vs = _rows(v, "v")
+        qp, qs, hq, qo = None, 0, 0, None
+        if q is not None:
+            qp, qs = _rows(q, "q")
+            hq = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            elif q_out.numel() != q.numel() or q_out.dtype != q.dtype:
+                raise ValueError("q_out must be like q")
+            qo = _dev(q_out, "q_out")
+        check(lib().gg_qk_norm_rope_append(self.handle, layer, qp, qs, kp, ks, vp, vs, int(dtype_of(k)), n, hq, wq, wk, float(eps),
+                                           pos, axes, axis, freq, pairs, st, qo,
+                                           _dev(slot_mapping, "slot_mapping", torch.int32), _stream(stream)),
+              "gg_qk_norm_rope_append")
+        return q_out
 
     def read(self, layer: int, slot_mapping: torch.Tensor, dtype: Optional[torch.dtype] = None,
              out: Optional[tuple] = None, stream: Optional[torch.cuda.Stream] = None):

@@ -170,6 +170,57 @@ gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void* v,
                          gg_dtype_t src_dtype, const int32_t* slot_mapping,
                          int n_rows, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Norm of each query and key head and the rotation of their positions, in one pass: what a
+ * layer does to the projected rows before the append and the attention. Covers rope_f16
+ * (kernels/gollmgo_ops.cu:88-128) with a table of frequencies, per-head norms and several
+ * position axes.
+ *   Row t, head h:  y = x * rsqrt(mean(x^2) + eps) * weight   (a NULL weight: y = x)
+ *   then pairs j < num_pairs turn by theta = positions[pair_axis[j]][t] * inv_freq[j]:
+ *     (a, b) -> (a cos theta - b sin theta, b cos theta + a sin theta)
+ *     GG_ROPE_HALVES: a = y[j], b = y[j + num_pairs]; GG_ROPE_PAIRS: a = y[2j], b = y[2j + 1]
+ *   and dims past 2 * num_pairs stay as they are. Angles are formed and reduced in 64 bits
+ *   (any int32 position keeps its angle), all else is fp32, rounded once on output.
+ *   q, k        : device rows of dtype (F32/F16/BF16): head h of row t starts at element
+ *                 t * {q,k}_stride + h * head_dim, so slices of a fused projection are
+ *                 taken as they are (strides in elements, at least heads * head_dim)
+ *   q_out, k_out: device [n_rows][heads][head_dim] of dtype, contiguous. q_out may be q
+ *                 (and k_out k) where that is contiguous; other overlaps are not allowed.
+ *   positions   : device int32[num_axes][n_rows], num_axes 1..8
+ *   pair_axis   : HOST uint8[num_pairs], the axis of each pair (copied by the call), or
+ *                 NULL for axis 0
+ *   inv_freq    : device float[num_pairs], 2 * num_pairs <= head_dim <= 1024, num_pairs
+ *                 0..512
+ *   q_weight, k_weight: device [head_dim] of dtype, or NULL; eps >= 0, finite
+ * num_q_heads or num_kv_heads may be 0 (the other side alone; its pointers are not used). */
+typedef enum {
+    GG_ROPE_HALVES = 0,
+    GG_ROPE_PAIRS = 1,
+} gg_rope_style_t;
+
+gg_status_t gg_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride,
+                            gg_dtype_t dtype, int n_rows, int num_q_heads, int num_kv_heads,
+                            int head_dim, const void* q_weight, const void* k_weight, float eps,
+                            const int32_t* positions, int num_axes, const uint8_t* pair_axis,
+                            const float* inv_freq, int num_pairs, gg_rope_style_t style,
+                            void* q_out, void* k_out, void* stream);
+
+/* The same with the keys written to a cache instead of k_out, and the values (v, strided as
+ * k) beside them, in the same launch: row t's goes to slot_mapping[t] (int32[n_rows];
+ * negative or past the pool: its K/V are skipped, its q is still written). The pool's kv
+ * heads and head_dim are the keys'. The pool holds what gg_kv_append would make of the fp32
+ * keys (their only rounding is the pool's). Pools of every type but PER_BLOCK INT8, whose
+ * scales belong to a block and not to a row: GG_ERR_INVALID (gg_qk_norm_rope, then
+ * gg_kv_append). Two rows of one call must not share a slot. */
+gg_status_t gg_qk_norm_rope_append(gg_kv_t kv, int layer, const void* q, long long q_stride,
+                                   const void* k, long long k_stride, const void* v,
+                                   long long v_stride, gg_dtype_t dtype, int n_rows,
+                                   int num_q_heads, const void* q_weight, const void* k_weight,
+                                   float eps, const int32_t* positions, int num_axes,
+                                   const uint8_t* pair_axis, const float* inv_freq, int num_pairs,
+                                   gg_rope_style_t style, void* q_out,
+                                   const int32_t* slot_mapping, void* stream);
+
 /* Read rows of one layer back as numbers: row i of k_out / v_out (device
  * [n_rows][num_kv_heads][head_dim] of out_dtype F32/F16/BF16; either may be NULL) is what
  * the pool holds in slot_mapping[i], its scales applied in fp32 and rounded once. For

@@ -41,3 +41,30 @@ def test_rule_holds_zero_and_half_steps(seed):
     assert (v[:, 3] == 0).all()
     assert ((s.view(np.uint32) & 0x7FFFF) == 0).all()
     assert (s <= (x.max(-1).clip(0) - x.min(-1).clip(None, 0)) / 15 * (1 + 1 / 16) * (1 + 2.0 ** -20)).all()
+
+
+def rope_call(**kw):
+    a = dict(q=1, qs=256, k=1, ks=128, dt=int(DType.F32), n=4, hq=4, hk=2, d=64, wq=None, wk=None, eps=1e-6, pos=1, axes=1,
+             axis=None, freq=1, pairs=32, style=0, qo=1, ko=1, stream=None)
+    a.update(kw)
+    return _lib.lib().gg_qk_norm_rope(*a.values())
+
+
+@pytest.mark.parametrize("bad,word", [
+    (dict(dt=int(DType.INT4)), "dtype"), (dict(n=-1), "n_rows"), (dict(n=(1 << 24) + 1), "n_rows"), (dict(hq=0, hk=0), "head count"),
+    (dict(hq=-1), "head count"), (dict(d=0), "head_dim"), (dict(d=1025, qs=9999, ks=9999), "head_dim"), (dict(pairs=33), "num_pairs"),
+    (dict(pairs=-1), "num_pairs"), (dict(axes=0), "num_axes"), (dict(axes=9), "num_axes"), (dict(style=2), "style"),
+    (dict(eps=float("nan")), "eps"), (dict(eps=-1e-9), "eps"), (dict(qs=255), "overlap"), (dict(ks=127), "overlap"),
+    (dict(q=None), "NULL"), (dict(qo=None), "NULL"), (dict(k=None), "NULL"), (dict(ko=None), "NULL"), (dict(pos=None), "NULL"),
+    (dict(freq=None), "NULL"), (dict(axis=(C.c_uint8 * 32)(*[1] * 32)), "pair_axis"),
+])
+def test_norm_rope_refuses_before_any_device_call(bad, word):
+    assert rope_call(**bad) == Status.ERR_INVALID
+    assert word in _lib.last_error()
+
+
+def test_norm_rope_append_refuses_no_handle():
+    lib = _lib.lib()
+    assert lib.gg_qk_norm_rope_append(None, 0, 1, 256, 1, 128, 1, 128, 0, 4, 4, None, None, 1e-6, 1, 1, None, 1, 32, 0, 1, 1,
+                                      None) == Status.ERR_INVALID
+    assert "kv is NULL" in _lib.last_error()
