@@ -1,0 +1,111 @@
+// int4_tile.h — sixteen rows of one kv head quantised into a 4-bit pool by a 256-thread workgroup: the
+// step that gg_kv_append and gg_qk_norm_rope_append share.
+//
+// LPR lanes hold a row, two runs of four dims each (16 rows of one head at LPR 16, of two heads at 8;
+// at 32 two rounds of eight rows). K rows go out as they are, two bytes a run. A V tile is [D/2][16]
+// with a token to a byte: sixteen rows that are one block in order meet in LDS and go out in 16-byte
+// runs, whole lines; other rows as bytes. Written as bytes throughout, a prompt of 32768 rows pays a
+// partial line for every byte.
+#pragma once
+#include "int4.h"
+#include "lanes.h"
+
+#include <type_traits>
+
+namespace gg {
+
+constexpr int int4_tile_head_group(int head_dim) { return head_dim == 64 ? 2 : 1; }  // heads of a workgroup
+// Groups of sixteen rows: one more than the rows fill, as the first block may be entered anywhere.
+inline unsigned int4_tile_groups(int n_rows) { return (unsigned)((n_rows + 15 + 15) / 16); }
+inline unsigned int4_tile_heads(int heads, int head_dim) {
+    const int g = int4_tile_head_group(head_dim);
+    return (unsigned)((heads + g - 1) / g);
+}
+
+// Calls f with the type as a constant.
+template <class F>
+inline void with_float(gg_dtype_t t, F f) {
+    switch (t) {
+        case GG_DTYPE_F32: f(std::integral_constant<gg_dtype_t, GG_DTYPE_F32>{}); break;
+        case GG_DTYPE_F16: f(std::integral_constant<gg_dtype_t, GG_DTYPE_F16>{}); break;
+        default: f(std::integral_constant<gg_dtype_t, GG_DTYPE_BF16>{}); break;
+    }
+}
+
+#ifdef __HIPCC__
+template <int LPR>
+struct Int4Tile {
+    static constexpr int kD = 8 * LPR;
+    static constexpr int kHeads = LPR == 8 ? 2 : 1;
+    __align__(16) uint8_t v[kHeads][kD / 2 * 16];
+};
+
+// Four codes in 16 bits.
+__device__ __forceinline__ uint32_t int4_codes4(const float (&x)[4], const Int4Scale& p) {
+    return int4_code(x[0], p) | (int4_code(x[1], p) << 4) | (int4_code(x[2], p) << 8) | (int4_code(x[3], p) << 12);
+}
+
+// Group `group` of rows and head group `hg`. get(r, h, u, ka, kb, va, vb, oa, ob): row r, head h, unit
+// u: the key's runs of dims oa .. oa + 3 and ob .. ob + 3 and the value's of 4u .. and D/2 + 4u .. . It
+// is called with every lane of a row or none.
+template <int LPR, class GET>
+__device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t* slots, int n_rows, int group, int hg,
+                                               Int4Tile<LPR>& tile, GET get) {
+    constexpr int D = Int4Tile<LPR>::kD, kRows = 256 / LPR;
+    constexpr int kRounds = LPR == 32 ? 2 : 1;
+    // A prompt's groups start where its blocks do (rows that are not a prompt's may be grouped anyhow).
+    const int s0 = slots[0];
+    const int r0 = group * 16 - (s0 < 0 ? 0 : s0 % p.bs % 16);
+    const int lead = slots[min(max(r0, 0), n_rows - 1)];
+    bool in_order = p.bs == 16 && r0 >= 0 && lead >= 0 && lead % 16 == 0;
+    const int u = threadIdx.x % LPR;
+#pragma unroll
+    for (int round = 0; round < kRounds; ++round) {
+        const int row = (round * kRows + (int)threadIdx.x / LPR) & 15, r = r0 + row;
+        const int slot = r >= 0 && r < n_rows ? slots[r] : -1;
+        in_order = in_order && slot == lead + row;
+    }
+    const bool whole = __syncthreads_and(in_order && lead + 15 < p.num_slots) != 0;
+#pragma unroll
+    for (int round = 0; round < kRounds; ++round) {
+        const int i = round * kRows + threadIdx.x / LPR, row = i & 15, hl = i >> 4;
+        const int r = r0 + row, h = hg * Int4Tile<LPR>::kHeads + hl;
+        const int slot = r >= 0 && r < n_rows && h < p.Hkv ? slots[r] : -1;
+        if (slot >= 0 && slot < p.num_slots) {
+            float ka[4], kb[4], va[4], vb[4];
+            int oa, ob;
+            get(r, h, u, ka, kb, va, vb, oa, ob);
+            float klo = 0.f, khi = 0.f, vlo = 0.f, vhi = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ka[e] = int4_clean(ka[e]), kb[e] = int4_clean(kb[e]), va[e] = int4_clean(va[e]), vb[e] = int4_clean(vb[e]);
+                klo = fminf(klo, fminf(ka[e], kb[e]));
+                khi = fmaxf(khi, fmaxf(ka[e], kb[e]));
+                vlo = fminf(vlo, fminf(va[e], vb[e]));
+                vhi = fmaxf(vhi, fmaxf(va[e], vb[e]));
+            }
+            const Int4Scale ks = int4_scale(group_min<LPR>(klo), group_max<LPR>(khi));
+            const Int4Scale vs = int4_scale(group_min<LPR>(vlo), group_max<LPR>(vhi));
+            const int blk = slot / p.bs, off = slot % p.bs;
+            uint8_t* kt = p.kc + p.tile0(blk, h) + (size_t)off * (D / 2);
+            *(uint16_t*)(kt + oa / 2) = (uint16_t)int4_codes4(ka, ks);
+            *(uint16_t*)(kt + ob / 2) = (uint16_t)int4_codes4(kb, ks);
+            uint8_t* vt = p.vc + p.tile0(blk, h) + off;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint8_t b = (uint8_t)(int4_code(va[e], vs) | (int4_code(vb[e], vs) << 4));
+                if (whole) tile.v[hl][(4 * u + e) * 16 + row] = b;
+                else vt[(size_t)(4 * u + e) * p.bs] = b;
+            }
+            if (u == 0) p.words[p.word(blk, h, off)] = ks.half | (vs.half << 16);
+        }
+    }
+    if (!whole) return;
+    __syncthreads();
+    const int hl = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2), h = hg * Int4Tile<LPR>::kHeads + hl;
+    if (hl < Int4Tile<LPR>::kHeads && h < p.Hkv)
+        *(uint4*)(p.vc + p.tile0(lead / 16, h) + (size_t)i * 16) = *(const uint4*)(tile.v[hl] + i * 16);
+}
+#endif
+
+}  // namespace gg

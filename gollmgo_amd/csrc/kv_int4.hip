@@ -3,6 +3,8 @@
 #include "gg_common.h"
 #include "attention_common.h"
 #include "int4.h"
+#include "int4_tile.h"
+#include "lanes.h"
 
 namespace gg {
 namespace {
@@ -18,6 +20,83 @@ __global__ void __launch_bounds__(256) append_int4_rows_kernel(Int4View p, const
     const size_t at = ((size_t)r * p.Hkv + h) * p.D;
     int4_write_row(p, slot / p.bs, h, slot % p.bs, [&](int d) { return load_as_f32(k, src, at + d); },
                    [&](int d) { return load_as_f32(v, src, at + d); });
+}
+
+// Sixteen rows of one head (or of 16 / LPR heads) per 256-thread workgroup: int4_tile.h.
+template <gg_dtype_t SRC, int LPR>
+__global__ void __launch_bounds__(256) append_int4_tile_kernel(Int4View p, const void* k, const void* v, const int32_t* slots,
+                                                               int n_rows) {
+    __shared__ Int4Tile<LPR> tile;
+    const size_t stride = (size_t)p.Hkv * p.D;
+    int4_tile_rows<LPR>(p, slots, n_rows, blockIdx.x, blockIdx.y, tile, [&](int r, int h, int u, float (&ka)[4], float (&kb)[4], float (&va)[4],
+                                                                           float (&vb)[4], int& oa, int& ob) {
+        const size_t at = (size_t)r * stride + (size_t)h * p.D;
+        oa = 4 * u;
+        ob = p.D / 2 + 4 * u;
+        const auto ra = load4<SRC>(k, at + oa), rb = load4<SRC>(k, at + ob), sa = load4<SRC>(v, at + oa), sb = load4<SRC>(v, at + ob);
+        to_f32<SRC>(ra, ka);
+        to_f32<SRC>(rb, kb);
+        to_f32<SRC>(sa, va);
+        to_f32<SRC>(sb, vb);
+    });
+}
+
+// A 4-bit pool's rows back, sixteen of one head per workgroup of 2 * head_dim threads: thread (row,
+// c) gives dims 8c .. 8c + 7. Where the rows are a block in order its V tile comes in whole 16-byte
+// runs through LDS (each run is sixteen tokens of two dims); else V byte by byte.
+template <gg_dtype_t DST, int D>
+__global__ void __launch_bounds__(2 * D) read_int4_tile_kernel(Int4View p, void* k_out, void* v_out, const int32_t* slots, int n_rows) {
+    constexpr int kC = D / 8;
+    __shared__ uint32_t s_v[D / 2 * 4 + D / 16];  // run i at word 4 i + i / 8 (eight runs apart: other banks)
+    const int h = blockIdx.y, row = threadIdx.x / kC, c = threadIdx.x % kC;
+    const int first = slots[0] < 0 ? 0 : slots[0] % p.bs;  // a prompt's groups start where its blocks do
+    const int r = (int)blockIdx.x * 16 - first % 16 + row;
+    const int slot = r >= 0 && r < n_rows ? slots[r] : -1;
+    const bool live = slot >= 0 && slot < p.num_slots;
+    const int blk = live ? slot / p.bs : 0, off = live ? slot % p.bs : 0;
+    const int lead = slots[min(max((int)blockIdx.x * 16 - first % 16, 0), n_rows - 1)];
+    const bool whole = __syncthreads_and(live && p.bs == 16 && slot == lead + row && lead % 16 == 0) != 0;
+    const uint8_t* vt = p.vc + p.tile0(blk, h);
+    if (whole && v_out) {
+        if (threadIdx.x < D / 2) {
+            const uint4 x = *(const uint4*)(vt + (size_t)threadIdx.x * 16);
+            uint32_t* d = s_v + 4 * threadIdx.x + threadIdx.x / 8;
+            d[0] = x.x, d[1] = x.y, d[2] = x.z, d[3] = x.w;
+        }
+        __syncthreads();
+    }
+    if (!live) return;
+    const uint32_t w = p.words[p.word(blk, h, off)];
+    const size_t to = ((size_t)r * p.Hkv + h) * D + 8 * c;
+    auto put = [&](void* out, const float (&f)[8]) {
+        if constexpr (DST == GG_DTYPE_F32) {
+            ((float4*)((float*)out + to))[0] = make_float4(f[0], f[1], f[2], f[3]);
+            ((float4*)((float*)out + to))[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *(uint4*)((uint16_t*)out + to) =
+                make_uint4(pack2<DST>(f[0], f[1]), pack2<DST>(f[2], f[3]), pack2<DST>(f[4], f[5]), pack2<DST>(f[6], f[7]));
+        }
+    };
+    float f[8];
+    if (k_out) {
+        const uint32_t x = *(const uint32_t*)(p.kc + p.tile0(blk, h) + (size_t)off * (D / 2) + 4 * c);
+        const float s = int4_k_scale(w);
+        const int z = int4_k_zero(w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = s * (float)((int)((x >> (4 * e)) & 15u) - z);
+        put(k_out, f);
+    }
+    if (v_out) {
+        const float s = int4_v_scale(w);
+        const int z = int4_v_zero(w);
+        const int i0 = 8 * (c % (kC / 2)), shift = c < kC / 2 ? 0 : 4;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t b = whole ? ((const uint8_t*)(s_v + 4 * (i0 + e) + i0 / 8))[off] : vt[(size_t)(i0 + e) * p.bs + off];
+            f[e] = s * (float)((int)((b >> shift) & 15u) - z);
+        }
+        put(v_out, f);
+    }
 }
 
 // One thread per element, row after row: K rows are contiguous; V elements of a row lie bs apart.
@@ -39,6 +118,18 @@ __global__ void __launch_bounds__(256) read_rows_kernel(KVView kv, void* k_out, 
 gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* v, gg_dtype_t src, const int32_t* slots,
                                   int n_rows, hipStream_t s) {
     const Int4View p = int4_view(kv, layer);
+    // By tiles of sixteen rows: head_dims of 8, 16 or 32 lanes of eight dims, vector loads.
+    const size_t align = src == GG_DTYPE_F32 ? 16 : 8;
+    if ((p.D == 64 || p.D == 128 || p.D == 256) && (uintptr_t)k % align == 0 && (uintptr_t)v % align == 0) {
+        with_float(src, [&](auto t) {
+            constexpr gg_dtype_t T = decltype(t)::value;
+            const dim3 grid(int4_tile_groups(n_rows), int4_tile_heads(p.Hkv, p.D));
+            if (p.D == 64) append_int4_tile_kernel<T, 8><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
+            else if (p.D == 128) append_int4_tile_kernel<T, 16><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
+            else append_int4_tile_kernel<T, 32><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
+        });
+        return check_hip(hipGetLastError(), "kv_append launch");
+    }
     const long long waves = (long long)n_rows * p.Hkv;
     append_int4_rows_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(p, k, v, src, slots, n_rows);
     return check_hip(hipGetLastError(), "kv_append launch");
@@ -46,6 +137,18 @@ gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* 
 
 gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype_t dst, const int32_t* slots, int n_rows,
                            hipStream_t s) {
+    if (kv->dtype == GG_DTYPE_INT4 && (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) &&
+        (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0 && kv->num_kv_heads <= 65535) {
+        const Int4View p = int4_view(kv, layer);
+        const dim3 grid(int4_tile_groups(n_rows), p.Hkv);
+        with_float(dst, [&](auto t) {
+            constexpr gg_dtype_t T = decltype(t)::value;
+            if (p.D == 64) read_int4_tile_kernel<T, 64><<<grid, 128, 0, s>>>(p, k_out, v_out, slots, n_rows);
+            else if (p.D == 128) read_int4_tile_kernel<T, 128><<<grid, 256, 0, s>>>(p, k_out, v_out, slots, n_rows);
+            else read_int4_tile_kernel<T, 256><<<grid, 512, 0, s>>>(p, k_out, v_out, slots, n_rows);
+        });
+        return check_hip(hipGetLastError(), "kv_read launch");
+    }
     const KVView view = make_kv_view(kv, layer);
     const long long n = (long long)n_rows * view.Hkv * view.D;
     if ((n + 255) / 256 > 0x7fffffffLL) return fail(GG_ERR_INVALID, "gg_kv_read: too many elements for one call");

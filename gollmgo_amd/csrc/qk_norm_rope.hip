@@ -1,12 +1,20 @@
 // qk_norm_rope.hip — norm of each query and key head and the rotation of its positions, in one pass;
 // keys to a dense output or, with the values, to a cache.
+//
+// Bound: each element is read and written once and costs about ten operations, so a prompt is bound by
+// memory and a step's few rows by the launch. The angle is the dear part (a 64-bit product and
+// reduction, then sine and cosine: about 50 instructions a pair) and belongs to a row, not to a head:
+// lanes hold the same pairs for every head they go through and form their angles once.
 #include "gg_common.h"
 #include "int4.h"
+#include "int4_tile.h"
+#include "lanes.h"
 
 namespace gg {
 namespace {
 
 constexpr int kRowsMaxD = 1024;
+constexpr int kRopeWaves = 4096;  // waves that fill the machine (heads_per_wave)
 
 // cos and sin of position times frequency. The angle in turns, and its whole turns taken off, in 64
 // bits (at position 2^31 the product still keeps 2^-21 of a turn); the rest is exact enough in fp32.
@@ -43,13 +51,8 @@ __device__ __forceinline__ void pool_store(uint8_t* base, gg_dtype_t dt, size_t 
 
 // One wave per (row, head): any head_dim, pair count, style and alignment. The turned row goes
 // through LDS only where it is written to a 4-bit pool, whose scale needs all of it.
-__global__ void __launch_bounds__(256) qk_norm_rope_rows_kernel(RopeArgs a, PoolOut p) {
-    __shared__ float s_row[4][kRowsMaxD];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long i = (long long)blockIdx.x * 4 + wave;
-    const int heads = a.Hq + a.Hkv, D = a.D, P = a.pairs;
-    if (i >= (long long)a.n * heads) return;
-    const int t = (int)(i / heads), hh = (int)(i % heads);
+__device__ __forceinline__ void rows_wave(const RopeArgs& a, const PoolOut& p, int t, int hh, float* s_row) {
+    const int lane = threadIdx.x & 63, D = a.D, P = a.pairs;
     const bool is_q = hh < a.Hq;
     const int h = is_q ? hh : hh - a.Hq;
     const void* src = is_q ? a.q : a.k;
@@ -82,7 +85,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_rows_kernel(RopeArgs a, Pool
         return weight ? x * norm * load_as_f32(weight, a.dt, d) : x;
     };
     auto put = [&](int d, float y) {
-        if (to_int4) s_row[wave][d] = y;
+        if (to_int4) s_row[d] = y;
         else if (cached) pool_store(p.kc, p.dt, tile + (size_t)off * D + d, y, kinv);
         else store_from_f32(out, a.dt, to + d, y);
     };
@@ -104,13 +107,244 @@ __global__ void __launch_bounds__(256) qk_norm_rope_rows_kernel(RopeArgs a, Pool
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        int4_write_row(p.i4, blk, h, off, [&](int d) { return s_row[wave][d]; },
+        int4_write_row(p.i4, blk, h, off, [&](int d) { return s_row[d]; },
                        [&](int d) { return load_as_f32(a.v, a.dt, vat + d); });
     } else {
         const float vinv = p.dt == GG_DTYPE_FP8_E4M3 ? p.v_inv[h] : 1.f;
         for (int d = lane; d < D; d += 64)
             pool_store(p.vc, p.dt, tile + (size_t)d * p.bs + off, load_as_f32(a.v, a.dt, vat + d), vinv);
     }
+}
+
+__global__ void __launch_bounds__(256) qk_norm_rope_rows_kernel(RopeArgs a, PoolOut p) {
+    __shared__ float s_row[4][kRowsMaxD];
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int heads = a.Hq + a.Hkv;
+    if (i < (long long)a.n * heads) rows_wave(a, p, (int)(i / heads), (int)(i % heads), s_row[threadIdx.x >> 6]);
+}
+
+// ---- head_dims of whole eights up to 256: LPR lanes a row, eight dims a lane ----
+//
+// Lane u of a row holds two runs of four dims, at oa and ob, loaded and stored as vectors:
+//   HALVES, u < P / 4 : dims 4u .. and P + 4u .. (pairs 4u .. 4u + 3, both ends in the lane)
+//   PAIRS,  u < P / 4 : dims 8u .. and 8u + 4 .. (the same pairs)
+//   past the pairs    : eight dims that only the norm touches
+struct Unit {
+    int oa, ob;
+    bool live, turned;
+};
+__device__ __forceinline__ Unit unit_of(const RopeArgs& a, int u) {
+    const int P = a.pairs;
+    Unit x;
+    x.live = 8 * u < a.D;
+    x.turned = 4 * u < P;
+    const bool halves = a.style == GG_ROPE_HALVES && x.turned;
+    x.oa = halves ? 4 * u : 8 * u;
+    x.ob = halves ? P + 4 * u : 8 * u + 4;
+    return x;
+}
+// Pairs 4u .. 4u + 3 of row t (c = 1, s = 0 past the pairs).
+struct Turn {
+    float c[4], s[4];
+};
+__device__ __forceinline__ Turn turn4(const RopeArgs& a, const Unit& x, int u, int t) {
+    Turn r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        r.c[e] = 1.f;
+        r.s[e] = 0.f;
+        if (x.turned) turn_of(a.positions[(size_t)pair_axis(a, 4 * u + e) * a.n + t], a.inv_freq[4 * u + e], r.c[e], r.s[e]);
+    }
+    return r;
+}
+__device__ __forceinline__ void apply_turn(const RopeArgs& a, const Unit& x, const Turn& r, float (&fa)[4], float (&fb)[4]) {
+    if (!x.turned) return;
+    if (a.style == GG_ROPE_HALVES) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p = fa[e], q = fb[e];
+            fa[e] = p * r.c[e] - q * r.s[e];
+            fb[e] = q * r.c[e] + p * r.s[e];
+        }
+    } else {
+        auto two = [](float& p, float& q, float c, float s) {
+            const float x = p, y = q;
+            p = x * c - y * s;
+            q = y * c + x * s;
+        };
+        two(fa[0], fa[1], r.c[0], r.s[0]);
+        two(fa[2], fa[3], r.c[1], r.s[1]);
+        two(fb[0], fb[1], r.c[2], r.s[2]);
+        two(fb[2], fb[3], r.c[3], r.s[3]);
+    }
+}
+// A row's two runs, normed (w: the weight's runs; none where has is false).
+template <int LPR>
+__device__ __forceinline__ void norm_runs(const RopeArgs& a, bool has, const float (&wa)[4], const float (&wb)[4], float (&fa)[4],
+                                          float (&fb)[4]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
+    const float r = rsqrtf(group_sum<LPR>(sum) / (float)a.D + a.eps);
+    if (!has) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        fa[e] = fa[e] * r * wa[e];
+        fb[e] = fb[e] * r * wb[e];
+    }
+}
+template <gg_dtype_t T>
+__device__ __forceinline__ void weight_runs(const void* w, const Unit& x, float (&wa)[4], float (&wb)[4]) {
+    to_f32<T>(load4<T>(w, x.oa), wa);
+    to_f32<T>(load4<T>(w, x.ob), wb);
+}
+
+// Wave (t, part): heads [part * per, +per) of row t, 64 / LPR at a time; the first Hq heads are
+// queries. Rows of heads four steps ahead are in flight.
+template <gg_dtype_t T, int LPR>
+__device__ __forceinline__ void dense_wave(const RopeArgs& a, int t, int h0, int h1) {
+    constexpr int kRPW = 64 / LPR, kAhead = 4;
+    const int lane = threadIdx.x & 63, u = lane % LPR, sub = lane / LPR;
+    const Unit x = unit_of(a, u);
+    auto source = [&](int h) -> const uint8_t* {
+        const bool is_q = h < a.Hq;
+        const size_t at = (size_t)t * (is_q ? a.q_stride : a.k_stride) + (size_t)(is_q ? h : h - a.Hq) * a.D;
+        return (const uint8_t*)(is_q ? a.q : a.k) + at * dtype_bytes(T);
+    };
+    Raw4<T> ra[kAhead], rb[kAhead];
+    auto fetch = [&](int i, int h) {
+        ra[i].w = rb[i].w = make_uint4(0, 0, 0, 0);
+        if (h < h1 && x.live) {
+            const uint8_t* p = source(h);
+            ra[i] = load4<T>(p, x.oa);
+            rb[i] = load4<T>(p, x.ob);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(i, h0 + sub + i * kRPW);
+    float qa[4], qb[4], ka[4], kb[4];
+    const bool has_q = a.q_weight != nullptr, has_k = a.k_weight != nullptr;
+    if (has_q && x.live) weight_runs<T>(a.q_weight, x, qa, qb);
+    if (has_k && x.live) weight_runs<T>(a.k_weight, x, ka, kb);
+    const Turn r = turn4(a, x, u, t);
+    for (int hb = h0 + sub; hb - sub < h1; hb += kAhead * kRPW) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int h = hb + i * kRPW;
+            if (h - sub >= h1) break;
+            float fa[4], fb[4];
+            to_f32<T>(ra[i], fa);
+            to_f32<T>(rb[i], fb);
+            fetch(i, h + kAhead * kRPW);
+            const bool is_q = h < a.Hq;
+            float wa[4], wb[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                wa[e] = is_q ? qa[e] : ka[e];
+                wb[e] = is_q ? qb[e] : kb[e];
+            }
+            norm_runs<LPR>(a, is_q ? has_q : has_k, wa, wb, fa, fb);
+            apply_turn(a, x, r, fa, fb);
+            if (h < h1 && x.live) {
+                const size_t to = ((size_t)t * (is_q ? a.Hq : a.Hkv) + (is_q ? h : h - a.Hq)) * a.D;
+                void* out = is_q ? a.q_out : a.k_out;
+                store4<T>(out, to + x.oa, fa);
+                store4<T>(out, to + x.ob, fb);
+            }
+        }
+    }
+}
+
+template <gg_dtype_t T, int LPR>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeArgs a, int heads, int parts, int per) {
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int t = (int)(i / parts), part = (int)(i % parts);
+    if (t >= a.n) return;
+    dense_wave<T, LPR>(a, t, part * per, min(heads, part * per + per));
+}
+
+// The same into a 4-bit pool: the first q_blocks workgroups do the queries as above, the others
+// sixteen rows of a kv head (or two) each, as gg_kv_append does (int4_tile.h).
+template <gg_dtype_t T, int LPR>
+__global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4View p, int q_blocks, int parts, int per,
+                                                                int groups) {
+    __shared__ Int4Tile<LPR> tile;
+    if ((int)blockIdx.x < q_blocks) {
+        const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        const int t = (int)(i / parts), part = (int)(i % parts);
+        if (t >= a.n) return;
+        dense_wave<T, LPR>(a, t, part * per, min(a.Hq, part * per + per));
+        return;
+    }
+    const int b = (int)blockIdx.x - q_blocks;
+    float wa[4], wb[4];
+    const Unit x = unit_of(a, threadIdx.x % LPR);
+    if (a.k_weight) weight_runs<T>(a.k_weight, x, wa, wb);
+    int4_tile_rows<LPR>(p, a.slots, a.n, b % groups, b / groups, tile,
+                        [&](int t, int h, int u, float (&ka)[4], float (&kb)[4], float (&va)[4], float (&vb)[4], int& oa, int& ob) {
+                            const size_t at = (size_t)t * a.k_stride + (size_t)h * a.D, vat = (size_t)t * a.v_stride + (size_t)h * a.D;
+                            const auto ra = load4<T>(a.k, at + x.oa), rb = load4<T>(a.k, at + x.ob);
+                            const auto sa = load4<T>(a.v, vat + 4 * u), sb = load4<T>(a.v, vat + a.D / 2 + 4 * u);
+                            const Turn r = turn4(a, x, u, t);
+                            to_f32<T>(ra, ka);
+                            to_f32<T>(rb, kb);
+                            to_f32<T>(sa, va);
+                            to_f32<T>(sb, vb);
+                            norm_runs<LPR>(a, a.k_weight != nullptr, wa, wb, ka, kb);
+                            apply_turn(a, x, r, ka, kb);
+                            oa = x.oa;
+                            ob = x.ob;
+                        });
+}
+
+// Into the other pools: queries as above, keys and values a row and head a wave.
+template <gg_dtype_t T, int LPR>
+__global__ void __launch_bounds__(256) qk_norm_rope_pool_kernel(RopeArgs a, PoolOut p, int q_blocks, int parts, int per) {
+    __shared__ float s_row[4][kRowsMaxD];
+    if ((int)blockIdx.x < q_blocks) {
+        const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        const int t = (int)(i / parts), part = (int)(i % parts);
+        if (t < a.n) dense_wave<T, LPR>(a, t, part * per, min(a.Hq, part * per + per));
+        return;
+    }
+    const long long i = (long long)((int)blockIdx.x - q_blocks) * 4 + (threadIdx.x >> 6);
+    if (i < (long long)a.n * a.Hkv) rows_wave(a, p, (int)(i / a.Hkv), a.Hq + (int)(i % a.Hkv), s_row[threadIdx.x >> 6]);
+}
+
+// Heads of a row for one wave: all of them where the rows alone fill the machine (one set of angles
+// a row), else as few as bring the waves there.
+int heads_per_wave(int n, int heads, int rows_per_wave) {
+    const int steps = (heads + rows_per_wave - 1) / rows_per_wave;
+    const int parts = n >= kRopeWaves ? 1 : (kRopeWaves + n - 1) / n;
+    return (steps + parts - 1) / parts * rows_per_wave;
+}
+
+// Whether the vector kernels take the call.
+bool vectors_fit(const RopeArgs& a) {
+    const size_t align = a.dt == GG_DTYPE_F32 ? 16 : 8;
+    const long long unit = (long long)(align / dtype_bytes(a.dt));
+    auto ok = [&](const void* p) { return (uintptr_t)p % align == 0; };
+    return a.D % 8 == 0 && a.D <= 256 && a.pairs % 4 == 0 && a.q_stride % unit == 0 && a.k_stride % unit == 0 &&
+           a.v_stride % unit == 0 && ok(a.q) && ok(a.k) && ok(a.v) && ok(a.q_out) && ok(a.k_out) && ok(a.q_weight) &&
+           ok(a.k_weight);
+}
+
+template <gg_dtype_t T, int LPR>
+gg_status_t launch_vectors(const RopeArgs& a, const KV* kv, const PoolOut& p, hipStream_t s) {
+    const int heads = kv ? a.Hq : a.Hq + a.Hkv;
+    const int per = heads ? heads_per_wave(a.n, heads, 64 / LPR) : 1, parts = heads ? (heads + per - 1) / per : 0;
+    const long long blocks = ((long long)a.n * parts + 3) / 4;
+    const bool tiles = kv && kv->dtype == GG_DTYPE_INT4 && a.D == 8 * LPR;
+    const unsigned groups = int4_tile_groups(a.n);
+    const long long all = blocks + (!kv     ? 0
+                                    : tiles ? (long long)groups * int4_tile_heads(a.Hkv, a.D)
+                                            : ((long long)a.n * a.Hkv + 3) / 4);
+    if (all > 0x7fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+    const int some = parts > 0 ? parts : 1;
+    if (!kv) qk_norm_rope_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, heads, some, per);
+    else if (tiles) qk_norm_rope_int4_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p.i4, (int)blocks, some, per, (int)groups);
+    else qk_norm_rope_pool_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p, (int)blocks, some, per);
+    return check_hip(hipGetLastError(), "qk_norm_rope launch");
 }
 
 }  // namespace
@@ -128,6 +362,16 @@ gg_status_t launch_qk_norm_rope(const RopeArgs& a, KV* kv, int layer, hipStream_
             p.k_inv = (const float*)kv->k_scales + (size_t)layer * kv->scale_layer_elems + kv->num_kv_heads;
             p.v_inv = (const float*)kv->v_scales + (size_t)layer * kv->scale_layer_elems + kv->num_kv_heads;
         }
+    }
+    if (vectors_fit(a)) {
+        gg_status_t st = GG_OK;
+        with_float(a.dt, [&](auto t) {
+            constexpr gg_dtype_t T = decltype(t)::value;
+            st = a.D <= 64    ? launch_vectors<T, 8>(a, kv, p, s)
+                 : a.D <= 128 ? launch_vectors<T, 16>(a, kv, p, s)
+                              : launch_vectors<T, 32>(a, kv, p, s);
+        });
+        return st;
     }
     const long long waves = (long long)a.n * (a.Hq + a.Hkv);
     if ((waves + 3) / 4 > 0x7fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");

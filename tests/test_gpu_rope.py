@@ -108,7 +108,9 @@ def test_norm_rope_in_place_and_unaligned(gv, d, P):
     wide[:, 1:hq * d + 1] = q.view(n, -1)
     odd = torch.as_strided(wide, (n, hq, d), (hq * d + 3, d, 1), 1)
     qu, _ = gv.qk_norm_rope(odd, k, **kw)
-    assert torch.equal(qu, qo)
+    # (Another kernel: its sums run in another order.)
+    ref, mag = want(as_np(q), as_np(w[0]), 1e-6, pos, axis, freq, "halves")
+    assert (np.abs(as_np(qu) - ref) <= tolerance(ref, mag, d, 40 + n, "bf16")).all()
 
 
 def test_norm_rope_special_rows(gv):
