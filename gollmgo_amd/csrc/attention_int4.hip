@@ -20,12 +20,13 @@
 //               The result gives lane (g4, c16) row c16 and the 16 tokens of block g4.
 //   O += P . V  : those 16 tokens are the A operand as they are; the V tile [D/2][16] gives a lane 16
 //               tokens of dims i and i + D/2 in one 16-byte load, two column tiles.
-// Each token's scales and zero points are one word; a wave puts the chunk's 64 words through LDS (one
-// load a lane instead of sixteen).
+// Each token's scales and zero points are one word. A lane loads and decodes one token's and puts them
+// into LDS, from where every lane takes its sixteen (decoded by their readers they cost 100
+// instructions a chunk).
 //
-// p s_v is held in f16 in units of B 2^-15, B a power of two at or above every s_v the wave has seen
+// p s_v is held in f16 in units of B 2^-10, B a power of two at or above every s_v the wave has seen
 // (O is rescaled when it grows). Values whose scales lie up to 2^12 apart keep 11 bits down to
-// p = 2^-17 that way; a piece whose scales lie further apart is computed row by row in fp32. Each
+// p = 2^-12 that way, and half a step of 2^-35 B below; a piece whose scales lie further apart is computed row by row in fp32. Each
 // query row has a power of two of its own (its largest |q| in [2^7, 2^8)), so rows do not touch.
 // PREC (fp32 queries or outputs): queries and p s_v in two f16 parts each, 22 bits, and the zero points
 // are taken from the codes in the operands (f16, exact). Summed apart, codes and zero points leave a
@@ -38,6 +39,11 @@ namespace {
 
 constexpr int kI4Tok = 64;                // tokens of a chunk
 constexpr float kI4Spread = 4096.f;       // ratio of value scales that f16 probabilities take
+// A row's maximum moves only when a chunk exceeds it by 2^kI4Slack: exponentials up to 2^5 are as good
+// as up to 1, and O, which every new maximum would rescale (with sixteen rows to a wave, nearly every
+// chunk finds one), is left alone.
+constexpr float kI4Slack = 5.f;
+constexpr float kI4Unit = 1024.f;         // p s_v in units of B / kI4Unit: at most 2^15
 constexpr uint32_t kLoNib = 0x000f000fu, kHiNib = 0x00f000f0u;
 
 // Eight codes of a K dword as an MFMA operand: (n0, n4), 16 (n1, n5), (n2, n6), 16 (n3, n7).
@@ -62,7 +68,10 @@ struct Int4Shared {
     uint4 q[kParts][NT][kMM][64];   // B operands of S
     uint32_t qz[NT * 16];           // -sum q of a row, two f16 parts
     float qmul[NT * 16];            // the row's score multiplier, log2 domain
-    uint32_t words[kWaves][kI4Tok];
+    // The chunk's tokens, decoded by the lane that loaded each token's word.
+    float ks[kWaves][kI4Tok], vs[kWaves][kI4Tok];
+    uint32_t kz[kWaves][kI4Tok];                       // (z, z)
+    __align__(16) uint16_t vz[kWaves][kI4Tok];         // in the order of the V operands
     float m[kWaves][NT * 16], l[kWaves][NT * 16];
     int bad[kWaves];
     __align__(16) float o[kWaves][16][HD + 4];
@@ -255,7 +264,9 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
         for (int t = 0; t < 2 * kVT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    float bound = 0.f, vnorm = 0.f;   // B, and 2^15 / B (wave-uniform)
+    float bound = 0.f, vnorm = 0.f;   // B, and kI4Unit / B (wave-uniform)
+    // Token c16 of a block in the V operands: half c16 / 8, dwords (0, 2), (1, 3) of each four.
+    const int vz_at = 16 * g4 + 8 * (c16 >> 3) + 4 * ((c16 >> 2) & 1) + 2 * (c16 & 1) + ((c16 >> 1) & 1);
     float vs_min = 3.0e38f;           // smallest value scale of the lane's tokens
 
     for (int ch = wave_u; ch < nchunks; ch += kWaves) {
@@ -263,23 +274,19 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         const int tlane = tc + 16 * g4;  // first token of the lane's block
         const bool missing = bl_cur.v < 0;
 
-        // The chunk's words to LDS (this wave's own slots: its LDS operations run in order).
+        // The chunk's scales and zero points to LDS (this wave's own slots: its LDS operations run in
+        // order). Tokens behind the end and in missing blocks count as values of scale 0.
         {
-            __builtin_amdgcn_wave_barrier();
-            s.words[wave][lane] = wr;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            // Value scales past B: B grows, and what has been summed shrinks with it.
-            float vs = int4_v_scale(wr);
-            vs = !missing && tlane + c16 < ctx ? vs : 0.f;
+            const bool live = !missing && tlane + c16 < ctx;
+            const float vs = live ? int4_v_scale(wr) : 0.f;
             vs_min = vs > 0.f ? fminf(vs_min, vs) : vs_min;
             if (__builtin_expect(__any(vs > bound), 0)) {
+                // Value scales past B: B grows, and what has been summed shrinks with it.
                 const float top = wave_max(vs);
                 const float grown = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
                 const float f = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(bound / grown)));
                 bound = __uint_as_float(__builtin_amdgcn_readfirstlane((int)__float_as_uint(grown)));
-                vnorm = 32768.f / bound;
+                vnorm = kI4Unit / bound;
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt) {
                     oz[rt] *= f;
@@ -287,6 +294,15 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                     for (int t = 0; t < 2 * kVT; ++t) o[rt][t] *= f;
                 }
             }
+            __builtin_amdgcn_wave_barrier();
+            const uint32_t zk = wr & 15u;
+            s.ks[wave][lane] = int4_k_scale(wr);
+            s.vs[wave][lane] = vs * vnorm;
+            s.kz[wave][lane] = zk | (zk << 16);
+            s.vz[wave][vz_at] = (uint16_t)int4_v_zero(wr);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
 
         // ---- S^T = K . Q^T ----
@@ -300,10 +316,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             for (int t = 0; t < 4; ++t) sacc[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         uint32_t kz[4];  // zero point of the lane's token of S tile t, a pair
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint32_t z = s.words[wave][16 * (c16 >> 2) + 4 * t + (c16 & 3)] & 15u;
-            kz[t] = z | (z << 16);
-        }
+        for (int t = 0; t < 4; ++t) kz[t] = s.kz[wave][16 * (c16 >> 2) + 4 * t + (c16 & 3)];
 #pragma unroll
         for (int mm = 0; mm < kMM; ++mm) {
             uint4 qop[kParts][NT];
@@ -328,26 +341,17 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                 for (int rt = 0; rt < NT; ++rt)
                     sacc[rt][t] = mfma(make_uint4(kz[t], 0u, 0u, 0u), make_uint4(qz[rt], 0u, 0u, 0u), sacc[rt][t], false);
         }
-        uint32_t w[16];  // words of the lane's block
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint4 x = *(const uint4*)&s.words[wave][16 * g4 + 4 * t];
-            w[4 * t] = x.x, w[4 * t + 1] = x.y, w[4 * t + 2] = x.z, w[4 * t + 3] = x.w;
-        }
         load_k(bl_next);
 
         // ---- online softmax ----
         const bool need_mask = tc + kI4Tok - 1 >= first_masked || __any(missing);
         uint32_t pop[NT][kParts][8];
-        float ks[16], vs[16];
+        float ks[16], vs[16];  // of the lane's block
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            ks[i] = int4_k_scale(w[i]);
-            vs[i] = int4_v_scale(w[i]) * vnorm;
-        }
-        if (__builtin_expect(need_mask, 0)) {  // (stale words may hold any scale: 0 times it must be 0)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) vs[i] = !missing && tlane + i < ctx ? vs[i] : 0.f;
+        for (int t = 0; t < 4; ++t) {
+            const float4 x = *(const float4*)&s.ks[wave][16 * g4 + 4 * t], y = *(const float4*)&s.vs[wave][16 * g4 + 4 * t];
+            ks[4 * t] = x.x, ks[4 * t + 1] = x.y, ks[4 * t + 2] = x.z, ks[4 * t + 3] = x.w;
+            vs[4 * t] = y.x, vs[4 * t + 1] = y.y, vs[4 * t + 2] = y.z, vs[4 * t + 3] = y.w;
         }
 #pragma unroll
         for (int rt = 0; rt < NT; ++rt) {
@@ -362,18 +366,11 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
             for (int i = 1; i < 16; ++i) cmax = fmaxf(cmax, sc[i]);
             cmax = max_over_rows(cmax * qmul[rt]);
-            const float m_new = fmaxf(m_run[rt], cmax);
-            const float alpha = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
-            m_run[rt] = m_new;
-            float psum = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qmul[rt], -m_new));
-                psum += sc[i];
-                sc[i] *= vs[i];
-            }
-            l_run[rt] = l_run[rt] * alpha + psum;
-            if (__any(alpha != 1.f)) {
+            const float m_new = cmax > m_run[rt] + kI4Slack ? cmax : m_run[rt];
+            if (__any(m_new != m_run[rt])) {
+                const float alpha = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+                l_run[rt] *= alpha;
+                m_run[rt] = m_new;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float al = __shfl(alpha, 4 * g4 + i);
@@ -382,6 +379,14 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                     for (int t = 0; t < 2 * kVT; ++t) o[rt][t][i] *= al;
                 }
             }
+            float psum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qmul[rt], -m_run[rt]));
+                psum += sc[i];
+                sc[i] *= vs[i];
+            }
+            l_run[rt] += psum;
             // Operand order of a V dword: tokens (0, 2), (1, 3).
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -398,14 +403,11 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         const typename IO::RawBlocks raw_after = IO::fetch_blocks(a, d.b, d.t0, ch + 2 * kWaves);
 
         // ---- O += P . V, the zero points as one more column tile ----
-        uint32_t vz[2][4];  // zero points in operand order
+        uint32_t vz[2][4];  // zero points as V operands
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = 8 * half + 4 * (i >> 1) + (i & 1);  // tokens t, t + 2
-                vz[half][i] = __builtin_amdgcn_perm(w[t + 2], w[t], 0x07060302u) & kLoNib;
-            }
+            const uint4 x = *(const uint4*)&s.vz[wave][16 * g4 + 8 * half];
+            vz[half][0] = x.x, vz[half][1] = x.y, vz[half][2] = x.z, vz[half][3] = x.w;
             if constexpr (!PREC) {
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt) {
@@ -462,7 +464,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         int4_piece_by_rows<HD>(a, kv, d, rows, 16 * NT, &s.o[wave][0][0]);
         return;
     }
-    const float unit = bound * 512.f;  // codes in 2^-24, p s_v in B 2^-15
+    const float unit = bound * (0x1p24f / kI4Unit);  // codes in 2^-24
     for (int rt = 0; rt < NT; ++rt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

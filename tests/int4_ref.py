@@ -98,8 +98,8 @@ def attention_tolerance(q, K, k_span, scale, ref, mag, reach, least, q_dtype, ou
       - unless queries or outputs are fp32, codes and zero points are summed apart, in fp32, 32
         products to a step aligned to the largest and cut at 2^-24 of it (33 * 2^-24 < 2^-18): 2^-18
         of the sum of p 15 s_v for each of the two sums, and for the scores of 15 s_k sum |q|;
-      - p s_v in f16 in units of B 2^-15, B a power of two less than twice the largest s_v: its last
-        part ends at 2^-24, so half a step of 2^-40 B, 2^-39 of the largest range, for each key;
+      - p s_v in f16 in units of B 2^-10, B a power of two less than twice the largest s_v: its last
+        part ends at 2^-24, so half a step of 2^-35 B, 2^-34 of the largest range, for each key;
       - the output's own rounding."""
     fine = "f32" in (q_dtype, out_dtype)
     qf = np.where(np.isfinite(q), q, 0)
@@ -109,4 +109,4 @@ def attention_tolerance(q, K, k_span, scale, ref, mag, reach, least, q_dtype, ou
     rel = 2 * score + 2.0 ** -22 * peak + (2.0 ** -16 if fine else 2.0 ** -11 + 2.0 ** -16)
     half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[out_dtype]
     tiny = 2.0 ** -25 if out_dtype == "f16" else 1e-38
-    return rel * mag + (0 if fine else 2 * 2.0 ** -18 * reach) + 2.0 ** -39 * least + half * np.abs(ref) + tiny
+    return rel * mag + (0 if fine else 2 * 2.0 ** -18 * reach) + 2.0 ** -34 * least + half * np.abs(ref) + tiny
