@@ -33,6 +33,7 @@
 // rounding of 2^-20 of the row's range, which f16 probabilities hide and fp32 results would show;
 // subtracting is 64 + 16 * 4 instructions more a chunk.
 #include "attention_mfma.h"
+#include "lanes.h"
 
 namespace gg {
 namespace {
@@ -111,77 +112,90 @@ __device__ __forceinline__ void int4_piece_by_rows(const AttnArgs& a, const KVVi
     }
 }
 
-// The piece's queries into LDS as MFMA operands, scaled row by row.
+// The piece's queries: HD / 8 threads a row, eight dims (one K dword) each. Loaded before the piece's
+// keys and values (loads retire in order, so the staging then waits for these alone), and put into
+// LDS as MFMA operands, scaled row by row.
 template <int NT, int HD, bool PREC>
-__device__ __forceinline__ void int4_stage_q(const AttnArgs& a, const KVView& kv, const PieceDesc& d, int rows,
-                                             Int4Shared<NT, HD, PREC>& s) {
-    constexpr int kMM = HD / 32, kPer = HD / 8;  // threads of a row: eight dims (one K dword) each
-    const int G = a.num_q_heads / kv.Hkv;
-    const int ch = threadIdx.x % kPer;
+struct Int4Queries {
+    static constexpr int kPer = HD / 8, kStep = 256 / kPer, kIt = (16 * NT + kStep - 1) / kStep;
+    uint4 w[kIt][PREC ? 2 : 1];
+
+    __device__ __forceinline__ void load(const AttnArgs& a, const KVView& kv, const PieceDesc& d, int rows) {
+        const int G = a.num_q_heads / kv.Hkv;
 #pragma unroll
-    for (int r = threadIdx.x / kPer; r < 16 * NT; r += 256 / kPer) {
-        float f[8];
-        const bool live = r < rows;
-        const int j = live ? (d.row0 + r) / G : 0, g = live ? (d.row0 + r) % G : 0;
-        const size_t at = (((size_t)d.b * a.rows + j) * a.num_q_heads + (size_t)d.kvh * G + g) * HD + 8 * ch;
-        if (a.q_dtype == GG_DTYPE_F32) {
-            struct __attribute__((packed, aligned(4))) F4 { float4 v; };
-            const float4 x = ((const F4*)((const float*)a.q + at))[0].v, y = ((const F4*)((const float*)a.q + at))[1].v;
-            const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = v[e];
-        } else {
+        for (int it = 0; it < kIt; ++it) {
+            const int r = min((int)threadIdx.x / kPer + it * kStep, rows - 1);
+            const int j = (d.row0 + r) / G, g = (d.row0 + r) % G;
+            const size_t at = (((size_t)d.b * a.rows + j) * a.num_q_heads + (size_t)d.kvh * G + g) * HD + 8 * (threadIdx.x % kPer);
             struct __attribute__((packed, aligned(2))) U4 { uint4 v; };
-            const uint4 w4 = ((const U4*)((const uint16_t*)a.q + at))->v;
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint16_t h = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                f[e] = a.q_dtype == GG_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+            if (PREC && a.q_dtype == GG_DTYPE_F32) {
+                struct __attribute__((packed, aligned(4))) F4 { uint4 v; };
+                w[it][0] = ((const F4*)((const float*)a.q + at))[0].v;
+                w[it][PREC ? 1 : 0] = ((const F4*)((const float*)a.q + at))[1].v;
+            } else {
+                w[it][0] = ((const U4*)((const uint16_t*)a.q + at))->v;
             }
-        }
-        float mx = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            f[e] = live ? f[e] : 0.f;
-            mx = fmaxf(mx, fabsf(f[e]));  // (a NaN is passed over)
-        }
-#pragma unroll
-        for (int o = 1; o < kPer; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        int e2 = 8;
-        if (mx > 0.f && mx <= 3.402823466e38f) (void)frexpf(mx, &e2);
-        const int k = e2 - 8;
-        // Two factors: 2^-k alone may overflow.
-        const float s1 = ldexpf(1.f, -(k / 2)), s2 = ldexpf(1.f, -(k - k / 2));
-        // Operand order (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
-        float sum = 0.f;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const float down = p & 1 ? 0.0625f : 1.f, up = p & 1 ? 16.f : 1.f;
-            const float x = f[p] * s1 * s2 * down, y = f[p + 4] * s1 * s2 * down;
-            hi[p] = f16_pair(x, y);
-            const float hx = f16_bits_to_f32((uint16_t)hi[p]), hy = f16_bits_to_f32((uint16_t)(hi[p] >> 16));
-            sum += (hx + hy) * up;
-            if constexpr (PREC) {
-                lo[p] = f16_pair(x - hx, y - hy);
-                sum += (f16_bits_to_f32((uint16_t)lo[p]) + f16_bits_to_f32((uint16_t)(lo[p] >> 16))) * up;
-            }
-        }
-        const int slot = 16 * (ch / kMM) + (r & 15);
-        s.q[0][r >> 4][ch % kMM][slot] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (PREC) s.q[1][r >> 4][ch % kMM][slot] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-#pragma unroll
-        for (int o = 1; o < kPer; o <<= 1) sum += __shfl_xor(sum, o);
-        if (ch == 0) {
-            const float top = f16_bits_to_f32(f32_to_f16_bits(-sum));
-            s.qz[r] = f16_pair(top, -sum - top);
-            // (The codes are in units of 2^-24. Positive and finite: a hidden score times it stays -inf.)
-            const float mul = ldexpf(a.scale * kLog2e, k + 24);
-            s.qmul[r] = fminf(fmaxf(mul, 0x1p-126f), 3.0e38f);
         }
     }
-}
+
+    __device__ __forceinline__ void stage(const AttnArgs& a, int rows, Int4Shared<NT, HD, PREC>& s) const {
+        constexpr int kMM = HD / 32;
+        const int ch = threadIdx.x % kPer;
+#pragma unroll
+        for (int it = 0; it < kIt; ++it) {
+            const int r = threadIdx.x / kPer + it * kStep;
+            if (r >= 16 * NT) break;
+            float f[8];
+            const uint32_t x[4] = {w[it][0].x, w[it][0].y, w[it][0].z, w[it][0].w};
+            if (PREC && a.q_dtype == GG_DTYPE_F32) {
+                const uint4 y = w[it][PREC ? 1 : 0];
+                f[0] = __uint_as_float(x[0]), f[1] = __uint_as_float(x[1]), f[2] = __uint_as_float(x[2]), f[3] = __uint_as_float(x[3]);
+                f[4] = __uint_as_float(y.x), f[5] = __uint_as_float(y.y), f[6] = __uint_as_float(y.z), f[7] = __uint_as_float(y.w);
+            } else if (a.q_dtype == GG_DTYPE_BF16) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(e & 1 ? x[e >> 1] & 0xffff0000u : x[e >> 1] << 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = f16_bits_to_f32((uint16_t)(x[e >> 1] >> (16 * (e & 1))));
+            }
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[e] = r < rows ? f[e] : 0.f;
+                mx = fmaxf(mx, fabsf(f[e]));  // (a NaN is passed over)
+            }
+            mx = group_max<kPer>(mx);
+            int e2 = 8;
+            if (mx > 0.f && mx <= 3.402823466e38f) (void)frexpf(mx, &e2);
+            const int k = e2 - 8;
+            // Two factors: 2^-k alone may overflow.
+            const float s1 = ldexpf(1.f, -(k / 2)), s2 = ldexpf(1.f, -(k - k / 2));
+            // Operand order (0, 4), (1, 5) / 16, (2, 6), (3, 7) / 16.
+            float sum = 0.f;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const float down = p & 1 ? 0.0625f : 1.f, up = p & 1 ? 16.f : 1.f;
+                const float u = f[p] * s1 * s2 * down, v = f[p + 4] * s1 * s2 * down;
+                hi[p] = f16_pair(u, v);
+                const float hu = f16_bits_to_f32((uint16_t)hi[p]), hv = f16_bits_to_f32((uint16_t)(hi[p] >> 16));
+                sum += (hu + hv) * up;
+                if constexpr (PREC) lo[p] = f16_pair(u - hu, v - hv);
+            }
+            const int slot = 16 * (ch / kMM) + (r & 15);
+            s.q[0][r >> 4][ch % kMM][slot] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if constexpr (PREC) s.q[1][r >> 4][ch % kMM][slot] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            sum = group_sum<kPer>(sum);
+            if (ch == 0) {
+                const float top = f16_bits_to_f32(f32_to_f16_bits(-sum));
+                s.qz[r] = f16_pair(top, -sum - top);
+                // (The codes are in units of 2^-24. Positive and finite: a hidden score times it stays -inf.)
+                const float mul = ldexpf(a.scale * kLog2e, k + 24);
+                s.qmul[r] = fminf(fmaxf(mul, 0x1p-126f), 3.0e38f);
+            }
+        }
+    }
+};
 
 template <int NT, int HD, bool PREC>
 __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, const PieceDesc& d) {
@@ -228,6 +242,8 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                 kr[t][0] = x.x, kr[t][1] = x.y;
             }
         }
+    };
+    auto load_word = [&](const LaneBlocks bl) {
         wr = kv.words[((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * kBS + c16];
     };
     auto load_v = [&](const LaneBlocks bl) {
@@ -235,12 +251,15 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
         for (int i = 0; i < kVT; ++i) vr[i] = *(const uint4*)(p + i * 16 * kBS);
     };
+    Int4Queries<NT, HD, PREC> qs;
     const auto fb = IO::first_blocks(a, d);
+    qs.load(a, kv, d, rows);
     LaneBlocks bl_cur = IO::lane_blocks(kv, fb.r0, d.t_end), bl_next = IO::lane_blocks(kv, fb.r1, d.t_end);
     load_k(bl_cur);
+    load_word(bl_cur);
     load_v(bl_cur);
 
-    int4_stage_q<NT, HD, PREC>(a, kv, d, rows, s);
+    qs.stage(a, rows, s);
     __syncthreads();
 
     uint32_t qz[NT];
@@ -305,6 +324,8 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
 
+        const typename IO::RawBlocks raw_after = IO::fetch_blocks(a, d.b, d.t0, ch + 2 * kWaves);
+        const bool need_mask = tc + kI4Tok - 1 >= first_masked || __any(missing);
         // ---- S^T = K . Q^T ----
         // (The Q index is opaque, so that the LDS reads stay in the loop.)
         int qlane;
@@ -342,14 +363,15 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                     sacc[rt][t] = mfma(make_uint4(kz[t], 0u, 0u, 0u), make_uint4(qz[rt], 0u, 0u, 0u), sacc[rt][t], false);
         }
         load_k(bl_next);
+        load_word(bl_next);
 
         // ---- online softmax ----
-        const bool need_mask = tc + kI4Tok - 1 >= first_masked || __any(missing);
         uint32_t pop[NT][kParts][8];
         float ks[16], vs[16];  // of the lane's block
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float4 x = *(const float4*)&s.ks[wave][16 * g4 + 4 * t], y = *(const float4*)&s.vs[wave][16 * g4 + 4 * t];
+            const int at = 16 * g4 + 4 * t;
+            const float4 x = *(const float4*)&s.ks[wave][at], y = *(const float4*)&s.vs[wave][at];
             ks[4 * t] = x.x, ks[4 * t + 1] = x.y, ks[4 * t + 2] = x.z, ks[4 * t + 3] = x.w;
             vs[4 * t] = y.x, vs[4 * t + 1] = y.y, vs[4 * t + 2] = y.z, vs[4 * t + 3] = y.w;
         }
@@ -365,9 +387,11 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             float cmax = sc[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) cmax = fmaxf(cmax, sc[i]);
-            cmax = max_over_rows(cmax * qmul[rt]);
-            const float m_new = cmax > m_run[rt] + kI4Slack ? cmax : m_run[rt];
-            if (__any(m_new != m_run[rt])) {
+            cmax *= qmul[rt];
+            // (The row's maximum over its four lanes is taken only where one of them is past the slack.)
+            if (__any(cmax > m_run[rt] + kI4Slack)) {
+                cmax = max_over_rows(cmax);
+                const float m_new = cmax > m_run[rt] + kI4Slack ? cmax : m_run[rt];
                 const float alpha = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
                 l_run[rt] *= alpha;
                 m_run[rt] = m_new;
@@ -400,44 +424,39 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                             f16_pair(x - f16_bits_to_f32((uint16_t)h), y - f16_bits_to_f32((uint16_t)(h >> 16)));
                 }
         }
-        const typename IO::RawBlocks raw_after = IO::fetch_blocks(a, d.b, d.t0, ch + 2 * kWaves);
 
         // ---- O += P . V, the zero points as one more column tile ----
-        uint32_t vz[2][4];  // zero points as V operands
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const uint4 x = *(const uint4*)&s.vz[wave][16 * g4 + 8 * half];
-            vz[half][0] = x.x, vz[half][1] = x.y, vz[half][2] = x.z, vz[half][3] = x.w;
+            const uint4 z = *(const uint4*)&s.vz[wave][16 * g4 + 8 * half];
+            uint4 pa[NT][kParts];
+#pragma unroll
+            for (int rt = 0; rt < NT; ++rt)
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    const uint32_t* q = pop[rt][p] + 4 * half;
+                    pa[rt][p] = make_uint4(q[0], q[1], q[2], q[3]);
+                }
             if constexpr (!PREC) {
 #pragma unroll
-                for (int rt = 0; rt < NT; ++rt) {
-                    const uint32_t* q = pop[rt][0] + 4 * half;
-                    oz[rt] = mfma(make_uint4(q[0], q[1], q[2], q[3]),
-                                  make_uint4(vz[half][0], vz[half][1], vz[half][2], vz[half][3]), oz[rt], false);
-                }
+                for (int rt = 0; rt < NT; ++rt) oz[rt] = mfma(pa[rt][0], z, oz[rt], false);
             }
-        }
 #pragma unroll
-        for (int i = 0; i < kVT; ++i) {
-            const uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int i = 0; i < kVT; ++i) {
+                const uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
                 const uint32_t x = v[2 * half], y = v[2 * half + 1], x8 = x >> 8, y8 = y >> 8;
                 uint4 lo = make_uint4(x & kLoNib, x8 & kLoNib, y & kLoNib, y8 & kLoNib);
                 uint4 hi = make_uint4(x & kHiNib, x8 & kHiNib, y & kHiNib, y8 & kHiNib);
                 if constexpr (PREC) {
-                    const uint32_t* z = vz[half];
-                    lo = less_zero(lo, z[0], z[1], z[2], z[3]);
-                    hi = less_zero(hi, z[0] << 4, z[1] << 4, z[2] << 4, z[3] << 4);
+                    lo = less_zero(lo, z.x, z.y, z.z, z.w);
+                    hi = less_zero(hi, z.x << 4, z.y << 4, z.z << 4, z.w << 4);
                 }
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
                     for (int p = 0; p < kParts; ++p) {
-                        const uint32_t* q = pop[rt][p] + 4 * half;
-                        const uint4 pa = make_uint4(q[0], q[1], q[2], q[3]);
-                        o[rt][i] = mfma(pa, lo, o[rt][i], false);
-                        o[rt][i + kVT] = mfma(pa, hi, o[rt][i + kVT], false);
+                        o[rt][i] = mfma(pa[rt][p], lo, o[rt][i], false);
+                        o[rt][i + kVT] = mfma(pa[rt][p], hi, o[rt][i + kVT], false);
                     }
             }
         }
@@ -469,6 +488,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int rr = 4 * g4 + i, r = rt * 16 + rr;
+            if (r >= rows) break;
             float mx = s.m[0][r];
 #pragma unroll
             for (int u = 1; u < kWaves; ++u) mx = fmaxf(mx, s.m[u][r]);
