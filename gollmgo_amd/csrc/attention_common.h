@@ -148,8 +148,8 @@ struct AttnShape {
 // Head_dim 64, or more than 64 query rows per kv head. At head_dim 128 two row tiles and the
 // three bf16 parts of P fit half the register file, at head_dim 64 four do. (A longer group
 // list than the plan's 16-bit head field holds goes to the generic kernel.)
-// 4-bit pools at head_dim 64 or 128 and any row count are tiled the same way (attention_int4.hip), two
-// row tiles at most: `full` stands for row groups of 16 * nt there too.
+// 4-bit pools at head_dim 64 or 128 and any row count are tiled the same way (attention_int4.hip):
+// `full` stands for row groups of 16 * nt there too.
 inline bool attn_full_supported(const KV* kv, int rows, int num_q_heads) {
     const long long tiles = ((long long)(num_q_heads / kv->num_kv_heads) * rows + 15) / 16;
     return kv->block_size == 16 &&
@@ -159,14 +159,17 @@ inline bool attn_full_supported(const KV* kv, int rows, int num_q_heads) {
 inline AttnShape attn_shape(const KV* kv, int rows, int num_q_heads) {
     const int tiles = (num_q_heads / kv->num_kv_heads * rows + 15) / 16;
     if (!attn_full_supported(kv, rows, num_q_heads)) return {false, tiles, 1};
-    const int most = kv->head_dim == 64 && kv->dtype != GG_DTYPE_INT4 ? 4 : 2;
+    // (4-bit pools: three at head_dim 128; four spill there.)
+    const int most = kv->head_dim == 64 ? 4 : kv->dtype == GG_DTYPE_INT4 ? 3 : 2;
     const int groups = (tiles + most - 1) / most;
     return {true, (tiles + groups - 1) / groups, groups};
 }
 
-// The two for a pool: 4-bit ones take 64-token chunks, two workgroups per CU.
+// The two for a pool. 4-bit ones: two workgroups per CU; chunks of 64 tokens, of 32 from three row
+// tiles on, which halve the chunk's scores, probabilities and scales next to the O tiles.
+__host__ __device__ constexpr int int4_chunk_tokens(int nt) { return nt <= 2 ? 64 : 32; }
 inline int attn_kv_chunk_tokens(const KV* kv, int nt) {
-    return kv->dtype == GG_DTYPE_INT4 ? 64 : attn_chunk_tokens((int)dtype_bytes(kv->dtype), nt);
+    return kv->dtype == GG_DTYPE_INT4 ? int4_chunk_tokens(nt) : attn_chunk_tokens((int)dtype_bytes(kv->dtype), nt);
 }
 inline int attn_kv_occupancy(const KV* kv, int nt) {
     return kv->dtype == GG_DTYPE_INT4 ? 2 : attn_occupancy((int)dtype_bytes(kv->dtype), nt, kv->head_dim);

@@ -38,7 +38,6 @@
 namespace gg {
 namespace {
 
-constexpr int kI4Tok = 64;                // tokens of a chunk
 constexpr float kI4Spread = 4096.f;       // ratio of value scales that f16 probabilities take
 // A row's maximum moves only when a chunk exceeds it by 2^kI4Slack: exponentials up to 2^5 are as good
 // as up to 1, and O, which every new maximum would rescale (with sixteen rows to a wave, nearly every
@@ -65,14 +64,15 @@ __device__ __forceinline__ uint32_t f16_pair(float a, float b) { return cvt_pk_f
 
 template <int NT, int HD, bool PREC>
 struct Int4Shared {
+    static constexpr int kTok = int4_chunk_tokens(NT);
     static constexpr int kMM = HD / 32, kParts = PREC ? 2 : 1;
     uint4 q[kParts][NT][kMM][64];   // B operands of S
     uint32_t qz[NT * 16];           // -sum q of a row, two f16 parts
     float qmul[NT * 16];            // the row's score multiplier, log2 domain
     // The chunk's tokens, decoded by the lane that loaded each token's word.
-    float ks[kWaves][kI4Tok], vs[kWaves][kI4Tok];
-    uint32_t kz[kWaves][kI4Tok];                       // (z, z)
-    __align__(16) uint16_t vz[kWaves][kI4Tok];         // in the order of the V operands
+    float ks[kWaves][kTok], vs[kWaves][kTok];
+    uint32_t kz[kWaves][kTok];                       // (z, z)
+    __align__(16) uint16_t vz[kWaves][kTok];         // in the order of the V operands
     float m[kWaves][NT * 16], l[kWaves][NT * 16];
     int bad[kWaves];
     __align__(16) float o[kWaves][16][HD + 4];
@@ -199,8 +199,10 @@ struct Int4Queries {
 
 template <int NT, int HD, bool PREC>
 __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, const PieceDesc& d) {
-    using IO = PieceIO<GG_DTYPE_INT8, kI4Tok, HD>;  // (block ids of 64-token chunks)
-    constexpr int kMM = HD / 32, kVT = HD / 32;     // K operands of a token; 16-byte V loads of a lane
+    constexpr int kTok = int4_chunk_tokens(NT), kNS = kTok / 16, kN = 4 * kNS;  // a chunk's tokens, S tiles; a lane's tokens
+    using IO = PieceIO<GG_DTYPE_INT8, kTok, HD>;    // (block ids of chunks)
+    using Geom = Geo<1, kTok, HD>;                  // (tokens of lanes and S tiles)
+    constexpr int kMM = HD / 32, kVT = HD / 32;     // K operands of a token; V loads of a lane
     constexpr int kParts = PREC ? 2 : 1;
     constexpr int kKW = HD / 32;                    // dwords of a lane's K run
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c16 = lane & 15, g4 = lane >> 4;
@@ -211,7 +213,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
     const int rows = min(G * nrows - d.row0, 16 * NT);
     if (rows <= 0) return;
     const int first_masked = ctx - nrows;
-    const int nchunks = (d.t_end - d.t0 + kI4Tok - 1) / kI4Tok;
+    const int nchunks = (d.t_end - d.t0 + kTok - 1) / kTok;
     __shared__ Int4Shared<NT, HD, PREC> s;
 
     // The call's own rows in this piece: written first, by the whole workgroup. (Row groups write
@@ -226,14 +228,18 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         }
     }
 
-    uint32_t kr[4][kKW];   // K: S tile t, the lane's token of it
-    uint4 vr[kVT];         // V: 16 tokens of dims 16 i + c16 and that plus HD / 2
-    uint32_t wr;           // word of token `lane` of the chunk
+    // The lane's first token in the chunk (its P run); the token it decodes the scales of; its K rows.
+    const int run = 16 * Geom::bq(g4) + Geom::ob(g4);
+    const int own = run + (c16 & (kN - 1));
+    const int krow = 16 * Geom::bq(c16 >> 2) + Geom::ob(c16 >> 2) + (c16 & 3);  // of S tile 0; 4 t further of tile t
+    uint32_t kr[kNS][kKW];        // K: S tile t, the lane's token of it
+    uint32_t vr[kVT][kN / 4];     // V: the lane's tokens, dims 16 i + c16 and that plus HD / 2
+    uint32_t wr;                  // word of token `own`
     auto load_k = [&](const LaneBlocks bl) {
         const int blk = max(bl.k, 0);
-        const uint8_t* p = kv.kc + ((size_t)blk * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)(c16 & 3) * (HD / 2) + 4 * kKW * g4;
+        const uint8_t* p = kv.kc + ((size_t)blk * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)(krow & 15) * (HD / 2) + 4 * kKW * g4;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < kNS; ++t) {
             if constexpr (kKW == 4) {
                 const uint4 x = *(const uint4*)(p + t * 4 * (HD / 2));
                 kr[t][0] = x.x, kr[t][1] = x.y, kr[t][2] = x.z, kr[t][3] = x.w;
@@ -244,12 +250,20 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         }
     };
     auto load_word = [&](const LaneBlocks bl) {
-        wr = kv.words[((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * kBS + c16];
+        wr = kv.words[((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * kBS + (own & 15)];
     };
     auto load_v = [&](const LaneBlocks bl) {
-        const uint8_t* p = kv.vc + ((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)c16 * kBS;
+        const uint8_t* p = kv.vc + ((size_t)max(bl.v, 0) * kv.Hkv + d.kvh) * (size_t)(kBS * HD) + (size_t)c16 * kBS + Geom::ob(g4);
 #pragma unroll
-        for (int i = 0; i < kVT; ++i) vr[i] = *(const uint4*)(p + i * 16 * kBS);
+        for (int i = 0; i < kVT; ++i) {
+            if constexpr (kN == 16) {
+                const uint4 x = *(const uint4*)(p + i * 16 * kBS);
+                vr[i][0] = x.x, vr[i][1] = x.y, vr[i][2] = x.z, vr[i][3] = x.w;
+            } else {
+                const uint2 x = *(const uint2*)(p + i * 16 * kBS);
+                vr[i][0] = x.x, vr[i][1] = x.y;
+            }
+        }
     };
     Int4Queries<NT, HD, PREC> qs;
     const auto fb = IO::first_blocks(a, d);
@@ -284,19 +298,19 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         for (int t = 0; t < 2 * kVT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     float bound = 0.f, vnorm = 0.f;   // B, and kI4Unit / B (wave-uniform)
-    // Token c16 of a block in the V operands: half c16 / 8, dwords (0, 2), (1, 3) of each four.
-    const int vz_at = 16 * g4 + 8 * (c16 >> 3) + 4 * ((c16 >> 2) & 1) + 2 * (c16 & 1) + ((c16 >> 1) & 1);
+    // Token `own` in the V operands: of each eight, tokens (0, 2), (1, 3), (4, 6), (5, 7).
+    const int vz_at = (own & ~7) + (own & 4) + 2 * (own & 1) + ((own >> 1) & 1);
     float vs_min = 3.0e38f;           // smallest value scale of the lane's tokens
 
     for (int ch = wave_u; ch < nchunks; ch += kWaves) {
-        const int tc = d.t0 + ch * kI4Tok;
-        const int tlane = tc + 16 * g4;  // first token of the lane's block
+        const int tc = d.t0 + ch * kTok;
+        const int tlane = tc + run;
         const bool missing = bl_cur.v < 0;
 
         // The chunk's scales and zero points to LDS (this wave's own slots: its LDS operations run in
         // order). Tokens behind the end and in missing blocks count as values of scale 0.
         {
-            const bool live = !missing && tlane + c16 < ctx;
+            const bool live = !missing && tc + own < ctx;
             const float vs = live ? int4_v_scale(wr) : 0.f;
             vs_min = vs > 0.f ? fminf(vs_min, vs) : vs_min;
             if (__builtin_expect(__any(vs > bound), 0)) {
@@ -315,9 +329,9 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             }
             __builtin_amdgcn_wave_barrier();
             const uint32_t zk = wr & 15u;
-            s.ks[wave][lane] = int4_k_scale(wr);
-            s.vs[wave][lane] = vs * vnorm;
-            s.kz[wave][lane] = zk | (zk << 16);
+            s.ks[wave][own] = int4_k_scale(wr);
+            s.vs[wave][own] = vs * vnorm;
+            s.kz[wave][own] = zk | (zk << 16);
             s.vz[wave][vz_at] = (uint16_t)int4_v_zero(wr);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -325,19 +339,19 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         }
 
         const typename IO::RawBlocks raw_after = IO::fetch_blocks(a, d.b, d.t0, ch + 2 * kWaves);
-        const bool need_mask = tc + kI4Tok - 1 >= first_masked || __any(missing);
+        const bool need_mask = tc + kTok - 1 >= first_masked || __any(missing);
         // ---- S^T = K . Q^T ----
         // (The Q index is opaque, so that the LDS reads stay in the loop.)
         int qlane;
         asm("" : "=v"(qlane) : "0"(lane), "s"(ch));
-        f32x4 sacc[NT][4];
+        f32x4 sacc[NT][kNS];
 #pragma unroll
         for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) sacc[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        uint32_t kz[4];  // zero point of the lane's token of S tile t, a pair
+            for (int t = 0; t < kNS; ++t) sacc[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t kz[kNS];  // zero point of the lane's token of S tile t, a pair
 #pragma unroll
-        for (int t = 0; t < 4; ++t) kz[t] = s.kz[wave][16 * (c16 >> 2) + 4 * t + (c16 & 3)];
+        for (int t = 0; t < kNS; ++t) kz[t] = s.kz[wave][krow + 4 * t];
 #pragma unroll
         for (int mm = 0; mm < kMM; ++mm) {
             uint4 qop[kParts][NT];
@@ -346,7 +360,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt) qop[p][rt] = s.q[p][rt][mm][qlane];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
+            for (int t = 0; t < kNS; ++t) {
                 uint4 kop = k_operand8(kr[t][mm]);
                 if constexpr (PREC) kop = less_zero(kop, kz[t], kz[t] << 4, kz[t], kz[t] << 4);
 #pragma unroll
@@ -357,7 +371,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         }
         if constexpr (!PREC) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int t = 0; t < kNS; ++t)
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt)
                     sacc[rt][t] = mfma(make_uint4(kz[t], 0u, 0u, 0u), make_uint4(qz[rt], 0u, 0u, 0u), sacc[rt][t], false);
@@ -366,27 +380,27 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         load_word(bl_next);
 
         // ---- online softmax ----
-        uint32_t pop[NT][kParts][8];
-        float ks[16], vs[16];  // of the lane's block
+        uint32_t pop[NT][kParts][kN / 2];
+        float ks[kN], vs[kN];  // of the lane's tokens
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int at = 16 * g4 + 4 * t;
+        for (int t = 0; t < kNS; ++t) {
+            const int at = run + 4 * t;
             const float4 x = *(const float4*)&s.ks[wave][at], y = *(const float4*)&s.vs[wave][at];
             ks[4 * t] = x.x, ks[4 * t + 1] = x.y, ks[4 * t + 2] = x.z, ks[4 * t + 3] = x.w;
             vs[4 * t] = y.x, vs[4 * t + 1] = y.y, vs[4 * t + 2] = y.z, vs[4 * t + 3] = y.w;
         }
 #pragma unroll
         for (int rt = 0; rt < NT; ++rt) {
-            float sc[16];
+            float sc[kN];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] = sacc[rt][i >> 2][i & 3] * ks[i];
+            for (int i = 0; i < kN; ++i) sc[i] = sacc[rt][i >> 2][i & 3] * ks[i];
             if (__builtin_expect(need_mask, 0)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sc[i] = !missing && tlane + i <= row_pos[rt] ? sc[i] : -INFINITY;
+                for (int i = 0; i < kN; ++i) sc[i] = !missing && tlane + i <= row_pos[rt] ? sc[i] : -INFINITY;
             }
             float cmax = sc[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) cmax = fmaxf(cmax, sc[i]);
+            for (int i = 1; i < kN; ++i) cmax = fmaxf(cmax, sc[i]);
             cmax *= qmul[rt];
             // (The row's maximum over its four lanes is taken only where one of them is past the slack.)
             if (__any(cmax > m_run[rt] + kI4Slack)) {
@@ -405,7 +419,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             }
             float psum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < kN; ++i) {
                 sc[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qmul[rt], -m_run[rt]));
                 psum += sc[i];
                 sc[i] *= vs[i];
@@ -413,7 +427,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             l_run[rt] += psum;
             // Operand order of a V dword: tokens (0, 2), (1, 3).
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < kNS; ++q)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float x = sc[4 * q + e], y = sc[4 * q + e + 2];
@@ -427,8 +441,8 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 
         // ---- O += P . V, the zero points as one more column tile ----
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const uint4 z = *(const uint4*)&s.vz[wave][16 * g4 + 8 * half];
+        for (int half = 0; half < kNS / 2; ++half) {
+            const uint4 z = *(const uint4*)&s.vz[wave][run + 8 * half];
             uint4 pa[NT][kParts];
 #pragma unroll
             for (int rt = 0; rt < NT; ++rt)
@@ -443,8 +457,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             }
 #pragma unroll
             for (int i = 0; i < kVT; ++i) {
-                const uint32_t v[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-                const uint32_t x = v[2 * half], y = v[2 * half + 1], x8 = x >> 8, y8 = y >> 8;
+                const uint32_t x = vr[i][2 * half], y = vr[i][2 * half + 1], x8 = x >> 8, y8 = y >> 8;
                 uint4 lo = make_uint4(x & kLoNib, x8 & kLoNib, y & kLoNib, y8 & kLoNib);
                 uint4 hi = make_uint4(x & kHiNib, x8 & kHiNib, y & kHiNib, y8 & kHiNib);
                 if constexpr (PREC) {
@@ -574,10 +587,13 @@ void launch_prec(const AttnArgs& a, const KVView& kv, hipStream_t s) {
 gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s) {
     if (kv.D == 128) {
         if (sh.nt == 1) launch_prec<1, 128>(a, kv, s);
-        else launch_prec<2, 128>(a, kv, s);
+        else if (sh.nt == 2) launch_prec<2, 128>(a, kv, s);
+        else launch_prec<3, 128>(a, kv, s);
     } else {
         if (sh.nt == 1) launch_prec<1, 64>(a, kv, s);
-        else launch_prec<2, 64>(a, kv, s);
+        else if (sh.nt == 2) launch_prec<2, 64>(a, kv, s);
+        else if (sh.nt == 3) launch_prec<3, 64>(a, kv, s);
+        else launch_prec<4, 64>(a, kv, s);
     }
     return check_hip(hipGetLastError(), "verify_attention launch");
 }

@@ -250,6 +250,8 @@ SHAPES = [
     (128, 16, 4, 4, 2, [2, 3, 130], [2, 0, 3]),
     (64, 16, 8, 2, 5, [5, 257, 1200], None),
     (64, 16, 32, 2, 6, [700, 31], [6, 2]),
+    (64, 16, 16, 2, 8, [900, 8, 33], [8, 8, 5]),
+    (128, 16, 12, 2, 8, [1100, 9, 31], [8, 7, 1]),
     (80, 16, 4, 2, 3, [3, 100, 700], None),
     (128, 8, 4, 2, 2, [2, 70], None),
     (256, 16, 2, 1, 2, [90, 600], None),
