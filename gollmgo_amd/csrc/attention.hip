@@ -197,7 +197,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
         if (!sh.full || (long long)num_seqs * kv->num_kv_heads * sh.groups > 0x7fffffffLL)
             return {ATTN_SCHED_GRID, attn_generic_partition(kv, num_seqs, rows, num_q_heads, max_blocks)};
         const int tok = int4_chunk_tokens(sh.nt);
-        const bool narrow = (long long)max_blocks * kv->block_size <= tok * lpt_min_chunks(tok);
+        const bool narrow = (long long)max_blocks * kv->block_size <= tok * lpt_min_chunks_of(kv, tok);
         const bool ranked = num_seqs <= kLptMaxSeqs && (long long)num_seqs * kv->num_kv_heads * sh.groups <= (1 << 18);
         return {narrow || !ranked ? ATTN_SCHED_ITEMS : ATTN_SCHED_LPT, 0};
     }

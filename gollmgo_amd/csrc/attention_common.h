@@ -206,6 +206,9 @@ constexpr int kLptMaxSeqs = 1024;
 constexpr int kLptPieceNum = 2, kLptPieceDen = 1;  // items >= slots
 constexpr int kLptTSpan = 31;
 __host__ __device__ constexpr int lpt_min_chunks(int tok) { return tok == 64 ? 12 : 16; }
+//     4-bit pools at 8 / 12 chunks of 64: one sequence of 3000 keys 16.1 / 16.8 µs a planned call, 16
+//     of 512-4096 keys at head_dim 64 15.6 / 16.3, larger batches the same.
+inline int lpt_min_chunks_of(const KV* kv, int tok) { return kv->dtype == GG_DTYPE_INT4 && tok == 64 ? 8 : lpt_min_chunks(tok); }
 __host__ __device__ constexpr bool lpt_few_items(int slots, int num_seqs, int num_kv_heads) {
     return num_seqs * num_kv_heads < slots;
 }

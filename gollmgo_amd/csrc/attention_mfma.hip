@@ -172,7 +172,7 @@ __device__ __forceinline__ int lpt_place(int u, int rg, int units, int groups) {
 // operands are integers below 2^53 and no non-integer quotient comes within 2^-28 of one).
 // Per call, 64 sequences 9.4 -> 7.6 µs, one 6.7 -> 5.2.
 template <int N>
-__global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, int tok_log2, int slots, int pieces) {
+__global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, int tok_log2, int tmin, int slots, int pieces) {
     __shared__ __align__(16) int s_key[N];  // piece size in chunks (0: no work)
     __shared__ __align__(16) int s_cnt[N];  // pieces of the sequence over all kv heads
     __shared__ int s_nch[N], s_ctx[N], s_rows[N], s_first[N], s_pos[N], s_np[N];
@@ -188,7 +188,6 @@ __global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, i
     s_rows[b] = nrows;
     const double C = (double)(block_sum<N>((unsigned long long)nch, s_sum) * (unsigned long long)Hkv);
     const bool few = lpt_few_items(slots, B, Hkv);
-    const int tmin = lpt_min_chunks(tok);
     int T;
     if (few) {
         // Fewer items than slots: every long item has to be cut to fill the slots, into equal
@@ -416,9 +415,9 @@ gg_status_t launch_attn_plan(const AttnArgs& a, hipStream_t s) {
     const int heads = Hkv * sh.groups;
     const int tok = attn_kv_chunk_tokens(kv, sh.nt);
     const int pieces = lpt_pieces(a.sk_grid, a.num_seqs, heads);
-    const int tok_log2 = tok == 64 ? 6 : 5;
-    if (a.num_seqs <= 256) attn_lpt_plan_kernel<256><<<1, 256, 0, s>>>(a, heads, tok_log2, a.sk_grid, pieces);
-    else attn_lpt_plan_kernel<kLptMaxSeqs><<<1, kLptMaxSeqs, 0, s>>>(a, heads, tok_log2, a.sk_grid, pieces);
+    const int tok_log2 = tok == 64 ? 6 : 5, tmin = lpt_min_chunks_of(kv, tok);
+    if (a.num_seqs <= 256) attn_lpt_plan_kernel<256><<<1, 256, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces);
+    else attn_lpt_plan_kernel<kLptMaxSeqs><<<1, kLptMaxSeqs, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces);
     return check_hip(hipGetLastError(), "verify_attention plan launch");
 }
 
