@@ -299,6 +299,8 @@ static gg_status_t rope_args(RopeArgs& a, const char* who, const void* q, long l
     a.q_weight = q_weight;
     a.k_weight = k_weight;
     a.eps = eps;
+    a.inv_d = 1.0f / (float)head_dim;
+    a.axes = num_axes;
     a.positions = positions;
     a.inv_freq = inv_freq;
     a.pairs = num_pairs;

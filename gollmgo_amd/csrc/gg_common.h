@@ -86,7 +86,8 @@ struct RopeArgs {
     int n, Hq, Hkv, D;
     const void* q_weight;        // null: no norm
     const void* k_weight;
-    float eps;
+    float eps, inv_d;            // inv_d: 1 / D
+    int axes;
     const int32_t* positions;    // [axes][n]
     const float* inv_freq;
     int pairs;                   // P

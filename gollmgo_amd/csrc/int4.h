@@ -30,20 +30,24 @@ __device__ __forceinline__ float int4_div(float x, const Int4Scale& p) {
     return __builtin_fmaf(__builtin_fmaf(-q, p.s, x), p.inv, q);
 }
 
-// lo <= 0 <= hi: the row's extremes.
+// lo <= 0 <= hi: the row's extremes. The quotient by 15 as in int4_div; 1 / s from the hardware's
+// reciprocal (1 ulp) and one Newton step, which gives the correctly rounded one for each of the sixteen
+// significands s can have (the codes of rows with every one of them are tested bit for bit).
 __device__ __forceinline__ Int4Scale int4_scale(float lo, float hi) {
     Int4Scale p;
-    const float r = (hi - lo) / 15.0f;
+    const float d = hi - lo, q = d * (1.0f / 15.0f);
+    const float r = __builtin_fmaf(__builtin_fmaf(-q, 15.0f, d), 1.0f / 15.0f, q);
     p.s = fmaxf(__uint_as_float((__float_as_uint(r) + 0x7ffffu) & 0xfff80000u), 0x1p-100f);
-    p.inv = 1.0f / p.s;
+    const float y = __builtin_amdgcn_rcpf(p.s);
+    p.inv = __builtin_fmaf(__builtin_fmaf(-p.s, y, 1.0f), y, y);
     p.z = __builtin_rintf(int4_div(-lo, p));
     p.half = ((__float_as_uint(p.s) >> 19) << 4) | (uint32_t)(int)p.z;
     return p;
 }
 
-// (x: int4_clean)
+// (x: int4_clean, within the row's extremes, so that rint(x / s) + z is 0 at least and 16 at most.)
 __device__ __forceinline__ uint32_t int4_code(float x, const Int4Scale& p) {
-    return (uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(int4_div(x, p)) + p.z, 0.f, 15.f);
+    return (uint32_t)(int)fminf(__builtin_rintf(int4_div(x, p)) + p.z, 15.f);
 }
 
 // A token's word: K in the low half, V in the high half.

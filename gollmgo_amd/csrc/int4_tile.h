@@ -75,14 +75,29 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
             float ka[4], kb[4], va[4], vb[4];
             int oa, ob;
             get(r, h, u, ka, kb, va, vb, oa, ob);
-            float klo = 0.f, khi = 0.f, vlo = 0.f, vhi = 0.f;
+            float klo, khi, vlo, vhi;
+            auto extremes = [&] {
+                klo = khi = vlo = vhi = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                ka[e] = int4_clean(ka[e]), kb[e] = int4_clean(kb[e]), va[e] = int4_clean(va[e]), vb[e] = int4_clean(vb[e]);
-                klo = fminf(klo, fminf(ka[e], kb[e]));
-                khi = fmaxf(khi, fmaxf(ka[e], kb[e]));
-                vlo = fminf(vlo, fminf(va[e], vb[e]));
-                vhi = fmaxf(vhi, fmaxf(va[e], vb[e]));
+                for (int e = 0; e < 4; ++e) {
+                    klo = fminf(klo, fminf(ka[e], kb[e]));
+                    khi = fmaxf(khi, fmaxf(ka[e], kb[e]));
+                    vlo = fminf(vlo, fminf(va[e], vb[e]));
+                    vhi = fmaxf(vhi, fmaxf(va[e], vb[e]));
+                }
+            };
+            extremes();
+            // Values that the rule replaces (NaN, past 1e36) are looked for once per lane: a product with
+            // zero that is not zero, or an extreme past the end.
+            float odd = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                odd = __builtin_fmaf(ka[e], 0.f, __builtin_fmaf(kb[e], 0.f, __builtin_fmaf(va[e], 0.f, __builtin_fmaf(vb[e], 0.f, odd))));
+            if (__builtin_expect(__any(odd != 0.f || fmaxf(khi, vhi) > 1e36f || fminf(klo, vlo) < -1e36f), 0)) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    ka[e] = int4_clean(ka[e]), kb[e] = int4_clean(kb[e]), va[e] = int4_clean(va[e]), vb[e] = int4_clean(vb[e]);
+                extremes();
             }
             const Int4Scale ks = int4_scale(group_min<LPR>(klo), group_max<LPR>(khi));
             const Int4Scale vs = int4_scale(group_min<LPR>(vlo), group_max<LPR>(vhi));

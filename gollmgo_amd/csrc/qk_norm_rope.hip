@@ -143,7 +143,8 @@ __device__ __forceinline__ Unit unit_of(const RopeArgs& a, int u) {
     x.ob = halves ? P + 4 * u : 8 * u + 4;
     return x;
 }
-// Pairs 4u .. 4u + 3 of row t (c = 1, s = 0 past the pairs).
+// Pairs 4u .. 4u + 3 of row t (c = 1, s = 0 past the pairs). Positions and frequencies are all asked for
+// before the first angle is formed.
 struct Turn {
     float c[4], s[4];
 };
@@ -153,8 +154,20 @@ __device__ __forceinline__ Turn turn4(const RopeArgs& a, const Unit& x, int u, i
     for (int e = 0; e < 4; ++e) {
         r.c[e] = 1.f;
         r.s[e] = 0.f;
-        if (x.turned) turn_of(a.positions[(size_t)pair_axis(a, 4 * u + e) * a.n + t], a.inv_freq[4 * u + e], r.c[e], r.s[e]);
     }
+    if (!x.turned) return r;
+    const float4 f = *(const float4*)(a.inv_freq + 4 * u);
+    int pos[4];
+    if (a.axes == 1) {
+        pos[0] = pos[1] = pos[2] = pos[3] = a.positions[t];
+    } else {
+        const uint32_t ax = a.axis[u >> 1] >> (16 * (u & 1));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pos[e] = a.positions[(size_t)((ax >> (4 * e)) & 15u) * a.n + t];
+    }
+    const float freq[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) turn_of(pos[e], freq[e], r.c[e], r.s[e]);
     return r;
 }
 __device__ __forceinline__ void apply_turn(const RopeArgs& a, const Unit& x, const Turn& r, float (&fa)[4], float (&fb)[4]) {
@@ -185,7 +198,7 @@ __device__ __forceinline__ void norm_runs(const RopeArgs& a, bool has, const flo
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
-    const float r = rsqrtf(group_sum<LPR>(sum) / (float)a.D + a.eps);
+    const float r = rsqrtf(__builtin_fmaf(group_sum<LPR>(sum), a.inv_d, a.eps));
     if (!has) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -199,65 +212,100 @@ __device__ __forceinline__ void weight_runs(const void* w, const Unit& x, float 
     to_f32<T>(load4<T>(w, x.ob), wb);
 }
 
-// Wave (t, part): heads [part * per, +per) of row t, 64 / LPR at a time; the first Hq heads are
-// queries. Rows of heads four steps ahead are in flight.
+// Heads [h0, h1) of one side (queries or keys) of row t by one wave, 64 / LPR at a time, four steps in
+// flight. A turned element is r (x w cos +- x' w' sin), x' the pair's other end and r the head's norm:
+// the products of weights and cosines are formed once for all heads.
 template <gg_dtype_t T, int LPR>
-__device__ __forceinline__ void dense_wave(const RopeArgs& a, int t, int h0, int h1) {
+__device__ __forceinline__ void dense_side(const RopeArgs& a, const Unit& x, const Turn& r, const void* rows, long long stride,
+                                           const void* weight, void* out, int heads, int t, int h0, int h1) {
     constexpr int kRPW = 64 / LPR, kAhead = 4;
-    const int lane = threadIdx.x & 63, u = lane % LPR, sub = lane / LPR;
-    const Unit x = unit_of(a, u);
-    auto source = [&](int h) -> const uint8_t* {
-        const bool is_q = h < a.Hq;
-        const size_t at = (size_t)t * (is_q ? a.q_stride : a.k_stride) + (size_t)(is_q ? h : h - a.Hq) * a.D;
-        return (const uint8_t*)(is_q ? a.q : a.k) + at * dtype_bytes(T);
-    };
+    constexpr size_t kEB = T == GG_DTYPE_F32 ? 4 : 2;
+    const int sub = (threadIdx.x & 63) / LPR;
+    const uint8_t* src = (const uint8_t*)rows + ((size_t)t * stride + (size_t)(h0 + sub) * a.D) * kEB;
+    uint8_t* dst = (uint8_t*)out + (((size_t)t * heads + h0 + sub) * a.D) * kEB;
+    const int n = x.live ? h1 - h0 - sub : 0;  // the lane's heads: 0, kRPW, ... below n
+    const size_t step = (size_t)kRPW * a.D * kEB;
     Raw4<T> ra[kAhead], rb[kAhead];
     auto fetch = [&](int i, int h) {
         ra[i].w = rb[i].w = make_uint4(0, 0, 0, 0);
-        if (h < h1 && x.live) {
-            const uint8_t* p = source(h);
-            ra[i] = load4<T>(p, x.oa);
-            rb[i] = load4<T>(p, x.ob);
+        if (h < n) {
+            ra[i] = load4<T>(src, x.oa);
+            rb[i] = load4<T>(src, x.ob);
         }
+        src += step;
     };
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(i, h0 + sub + i * kRPW);
-    float qa[4], qb[4], ka[4], kb[4];
-    const bool has_q = a.q_weight != nullptr, has_k = a.k_weight != nullptr;
-    if (has_q && x.live) weight_runs<T>(a.q_weight, x, qa, qb);
-    if (has_k && x.live) weight_runs<T>(a.k_weight, x, ka, kb);
-    const Turn r = turn4(a, x, u, t);
-    for (int hb = h0 + sub; hb - sub < h1; hb += kAhead * kRPW) {
+    for (int i = 0; i < kAhead; ++i) fetch(i, i * kRPW);
+    float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
+    if (weight && x.live) weight_runs<T>(weight, x, wa, wb);
+    // Pair e of the lane's four: its ends' weights.
+    float c0[4], c1[4], s0[4], s1[4];  // (first end: x c0 - x' s0; second: x' c1 + x s1)
+    const bool halves = a.style == GG_ROPE_HALVES;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float w0 = halves ? wa[e] : e < 2 ? wa[2 * e] : wb[2 * (e & 1)];
+        const float w1 = halves ? wb[e] : e < 2 ? wa[2 * e + 1] : wb[2 * (e & 1) + 1];
+        c0[e] = w0 * r.c[e];
+        s1[e] = w0 * r.s[e];
+        c1[e] = w1 * r.c[e];
+        s0[e] = w1 * r.s[e];
+    }
+    for (int hb = 0; hb < h1 - h0; hb += kAhead * kRPW) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int h = hb + i * kRPW;
-            if (h - sub >= h1) break;
+            if (h >= h1 - h0) break;
             float fa[4], fb[4];
             to_f32<T>(ra[i], fa);
             to_f32<T>(rb[i], fb);
             fetch(i, h + kAhead * kRPW);
-            const bool is_q = h < a.Hq;
-            float wa[4], wb[4];
+            float k = 1.f;
+            if (weight) {
+                float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                wa[e] = is_q ? qa[e] : ka[e];
-                wb[e] = is_q ? qb[e] : kb[e];
+                for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
+                k = rsqrtf(__builtin_fmaf(group_sum<LPR>(sum), a.inv_d, a.eps));
             }
-            norm_runs<LPR>(a, is_q ? has_q : has_k, wa, wb, fa, fb);
-            apply_turn(a, x, r, fa, fb);
-            if (h < h1 && x.live) {
-                const size_t to = ((size_t)t * (is_q ? a.Hq : a.Hkv) + (is_q ? h : h - a.Hq)) * a.D;
-                void* out = is_q ? a.q_out : a.k_out;
-                store4<T>(out, to + x.oa, fa);
-                store4<T>(out, to + x.ob, fb);
+            if (!x.turned) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    fa[e] = fa[e] * wa[e] * k;
+                    fb[e] = fb[e] * wb[e] * k;
+                }
+            } else {
+                auto pair = [&](float& p, float& q, int e) {
+                    const float u = (p * c0[e] - q * s0[e]) * k, v = (q * c1[e] + p * s1[e]) * k;
+                    p = u;
+                    q = v;
+                };
+                if (halves) {
+                    pair(fa[0], fb[0], 0), pair(fa[1], fb[1], 1), pair(fa[2], fb[2], 2), pair(fa[3], fb[3], 3);
+                } else {
+                    pair(fa[0], fa[1], 0), pair(fa[2], fa[3], 1), pair(fb[0], fb[1], 2), pair(fb[2], fb[3], 3);
+                }
             }
+            if (h < n) {
+                store4<T>(dst, x.oa, fa);
+                store4<T>(dst, x.ob, fb);
+            }
+            dst += step;
         }
     }
 }
 
+// Wave (t, part): heads [h0, h1) of row t; the first Hq heads are queries.
+template <gg_dtype_t T, int LPR>
+__device__ __forceinline__ void dense_wave(const RopeArgs& a, int t, int h0, int h1) {
+    const int u = threadIdx.x % LPR;
+    const Unit x = unit_of(a, u);
+    const Turn r = turn4(a, x, u, t);
+    if (h0 < a.Hq) dense_side<T, LPR>(a, x, r, a.q, a.q_stride, a.q_weight, a.q_out, a.Hq, t, h0, min(h1, a.Hq));
+    if (h1 > a.Hq) dense_side<T, LPR>(a, x, r, a.k, a.k_stride, a.k_weight, a.k_out, a.Hkv, t, max(h0 - a.Hq, 0), h1 - a.Hq);
+}
+
 template <gg_dtype_t T, int LPR>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeArgs a, int heads, int parts, int per) {
-    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = (int)(i / parts), part = (int)(i % parts);
     if (t >= a.n) return;
     dense_wave<T, LPR>(a, t, part * per, min(heads, part * per + per));
@@ -270,7 +318,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4
                                                                 int groups) {
     __shared__ Int4Tile<LPR> tile;
     if ((int)blockIdx.x < q_blocks) {
-        const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int t = (int)(i / parts), part = (int)(i % parts);
         if (t >= a.n) return;
         dense_wave<T, LPR>(a, t, part * per, min(a.Hq, part * per + per));
@@ -302,7 +350,7 @@ template <gg_dtype_t T, int LPR>
 __global__ void __launch_bounds__(256) qk_norm_rope_pool_kernel(RopeArgs a, PoolOut p, int q_blocks, int parts, int per) {
     __shared__ float s_row[4][kRowsMaxD];
     if ((int)blockIdx.x < q_blocks) {
-        const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+        const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int t = (int)(i / parts), part = (int)(i % parts);
         if (t < a.n) dense_wave<T, LPR>(a, t, part * per, min(a.Hq, part * per + per));
         return;
@@ -326,7 +374,7 @@ bool vectors_fit(const RopeArgs& a) {
     auto ok = [&](const void* p) { return (uintptr_t)p % align == 0; };
     return a.D % 8 == 0 && a.D <= 256 && a.pairs % 4 == 0 && a.q_stride % unit == 0 && a.k_stride % unit == 0 &&
            a.v_stride % unit == 0 && ok(a.q) && ok(a.k) && ok(a.v) && ok(a.q_out) && ok(a.k_out) && ok(a.q_weight) &&
-           ok(a.k_weight);
+           ok(a.k_weight) && (uintptr_t)a.inv_freq % 16 == 0;
 }
 
 template <gg_dtype_t T, int LPR>
@@ -339,7 +387,7 @@ gg_status_t launch_vectors(const RopeArgs& a, const KV* kv, const PoolOut& p, hi
     const long long all = blocks + (!kv     ? 0
                                     : tiles ? (long long)groups * int4_tile_heads(a.Hkv, a.D)
                                             : ((long long)a.n * a.Hkv + 3) / 4);
-    if (all > 0x7fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+    if (all > 0x3fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
     const int some = parts > 0 ? parts : 1;
     if (!kv) qk_norm_rope_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, heads, some, per);
     else if (tiles) qk_norm_rope_int4_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p.i4, (int)blocks, some, per, (int)groups);
