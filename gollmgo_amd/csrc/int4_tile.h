@@ -2,10 +2,10 @@
 // step that gg_kv_append and gg_qk_norm_rope_append share.
 //
 // LPR lanes hold a row, two runs of four dims each (16 rows of one head at LPR 16, of two heads at 8;
-// at 32 two rounds of eight rows). K rows go out as they are, two bytes a run. A V tile is [D/2][16]
-// with a token to a byte: sixteen rows that are one block in order meet in LDS and go out in 16-byte
-// runs, whole lines; other rows as bytes. Written as bytes throughout, a prompt of 32768 rows pays a
-// partial line for every byte.
+// at 32 two rounds of eight rows). Sixteen rows that are one block in order meet in LDS, and the block's
+// K tile, V tile (a byte to a token) and words go out in 16-byte runs, whole lines; other rows go out
+// two bytes of K and single bytes of V at a time, each a partial line. Workgroups of one row group are
+// neighbours, so that whole source rows are read at a time.
 #pragma once
 #include "int4.h"
 #include "lanes.h"
@@ -37,7 +37,8 @@ template <int LPR>
 struct Int4Tile {
     static constexpr int kD = 8 * LPR;
     static constexpr int kHeads = LPR == 8 ? 2 : 1;
-    __align__(16) uint8_t v[kHeads][kD / 2 * 16];
+    __align__(16) uint8_t kv[kHeads][2][kD / 2 * 16];  // K tile, V tile
+    __align__(16) uint32_t words[kHeads][16];
 };
 
 // Four codes in 16 bits.
@@ -45,36 +46,51 @@ __device__ __forceinline__ uint32_t int4_codes4(const float (&x)[4], const Int4S
     return int4_code(x[0], p) | (int4_code(x[1], p) << 4) | (int4_code(x[2], p) << 8) | (int4_code(x[3], p) << 12);
 }
 
-// Group `group` of rows and head group `hg`. get(r, h, u, ka, kb, va, vb, oa, ob): row r, head h, unit
-// u: the key's runs of dims oa .. oa + 3 and ob .. ob + 3 and the value's of 4u .. and D/2 + 4u .. . It
-// is called with every lane of a row or none.
-template <int LPR, class GET>
+// A unit of a row as it was loaded: two runs of the key and two of the value.
+template <gg_dtype_t T>
+struct Int4Raw {
+    Raw4<T> ka, kb, va, vb;
+};
+
+// Group `group` of rows and head group `hg`. fetch(r, h, u) loads row r, head h, unit u (an Int4Raw): the
+// key's runs of dims oa .. oa + 3 and ob .. ob + 3 and the value's of 4u .. and D/2 + 4u .. ; it is
+// called before the row's slot is known. make(raw, r, h, u, ka, kb, va, vb, oa, ob) gives the values to be
+// stored, called with every lane of a row or none.
+template <gg_dtype_t T, int LPR, class FETCH, class MAKE>
 __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t* slots, int n_rows, int group, int hg,
-                                               Int4Tile<LPR>& tile, GET get) {
+                                               Int4Tile<LPR>& tile, FETCH fetch, MAKE make) {
     constexpr int D = Int4Tile<LPR>::kD, kRows = 256 / LPR;
     constexpr int kRounds = LPR == 32 ? 2 : 1;
     // A prompt's groups start where its blocks do (rows that are not a prompt's may be grouped anyhow).
     const int s0 = slots[0];
     const int r0 = group * 16 - (s0 < 0 ? 0 : s0 % p.bs % 16);
+    const int u = threadIdx.x % LPR;
+    Int4Raw<T> raw[kRounds];
+    int slot_of[kRounds];
     const int lead = slots[min(max(r0, 0), n_rows - 1)];
     bool in_order = p.bs == 16 && r0 >= 0 && lead >= 0 && lead % 16 == 0;
-    const int u = threadIdx.x % LPR;
+#pragma unroll
+    for (int round = 0; round < kRounds; ++round) {
+        const int i = round * kRows + threadIdx.x / LPR, r = r0 + (i & 15), h = hg * Int4Tile<LPR>::kHeads + (i >> 4);
+        slot_of[round] = slots[min(max(r, 0), n_rows - 1)];
+        raw[round] = fetch(min(max(r, 0), n_rows - 1), min(h, p.Hkv - 1), u);
+    }
 #pragma unroll
     for (int round = 0; round < kRounds; ++round) {
         const int row = (round * kRows + (int)threadIdx.x / LPR) & 15, r = r0 + row;
-        const int slot = r >= 0 && r < n_rows ? slots[r] : -1;
-        in_order = in_order && slot == lead + row;
+        if (r < 0 || r >= n_rows) slot_of[round] = -1;
+        in_order = in_order && slot_of[round] == lead + row;
     }
     const bool whole = __syncthreads_and(in_order && lead + 15 < p.num_slots) != 0;
 #pragma unroll
     for (int round = 0; round < kRounds; ++round) {
         const int i = round * kRows + threadIdx.x / LPR, row = i & 15, hl = i >> 4;
         const int r = r0 + row, h = hg * Int4Tile<LPR>::kHeads + hl;
-        const int slot = r >= 0 && r < n_rows && h < p.Hkv ? slots[r] : -1;
+        const int slot = h < p.Hkv ? slot_of[round] : -1;
         if (slot >= 0 && slot < p.num_slots) {
             float ka[4], kb[4], va[4], vb[4];
             int oa, ob;
-            get(r, h, u, ka, kb, va, vb, oa, ob);
+            make(raw[round], r, h, u, ka, kb, va, vb, oa, ob);
             float klo, khi, vlo, vhi;
             auto extremes = [&] {
                 klo = khi = vlo = vhi = 0.f;
@@ -102,24 +118,36 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
             const Int4Scale ks = int4_scale(group_min<LPR>(klo), group_max<LPR>(khi));
             const Int4Scale vs = int4_scale(group_min<LPR>(vlo), group_max<LPR>(vhi));
             const int blk = slot / p.bs, off = slot % p.bs;
-            uint8_t* kt = p.kc + p.tile0(blk, h) + (size_t)off * (D / 2);
-            *(uint16_t*)(kt + oa / 2) = (uint16_t)int4_codes4(ka, ks);
-            *(uint16_t*)(kt + ob / 2) = (uint16_t)int4_codes4(kb, ks);
-            uint8_t* vt = p.vc + p.tile0(blk, h) + off;
+            const uint32_t k01 = int4_codes4(ka, ks), k23 = int4_codes4(kb, ks), word = ks.half | (vs.half << 16);
+            uint32_t vb4[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint8_t b = (uint8_t)(int4_code(va[e], vs) | (int4_code(vb[e], vs) << 4));
-                if (whole) tile.v[hl][(4 * u + e) * 16 + row] = b;
-                else vt[(size_t)(4 * u + e) * p.bs] = b;
+            for (int e = 0; e < 4; ++e) vb4[e] = int4_code(va[e], vs) | (int4_code(vb[e], vs) << 4);
+            if (whole) {
+                *(uint16_t*)&tile.kv[hl][0][row * (D / 2) + oa / 2] = (uint16_t)k01;
+                *(uint16_t*)&tile.kv[hl][0][row * (D / 2) + ob / 2] = (uint16_t)k23;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tile.kv[hl][1][(4 * u + e) * 16 + row] = (uint8_t)vb4[e];
+                if (u == 0) tile.words[hl][row] = word;
+            } else {
+                uint8_t* kt = p.kc + p.tile0(blk, h) + (size_t)off * (D / 2);
+                *(uint16_t*)(kt + oa / 2) = (uint16_t)k01;
+                *(uint16_t*)(kt + ob / 2) = (uint16_t)k23;
+                uint8_t* vt = p.vc + p.tile0(blk, h) + off;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) vt[(size_t)(4 * u + e) * p.bs] = (uint8_t)vb4[e];
+                if (u == 0) p.words[p.word(blk, h, off)] = word;
             }
-            if (u == 0) p.words[p.word(blk, h, off)] = ks.half | (vs.half << 16);
         }
     }
     if (!whole) return;
     __syncthreads();
-    const int hl = threadIdx.x / (D / 2), i = threadIdx.x % (D / 2), h = hg * Int4Tile<LPR>::kHeads + hl;
-    if (hl < Int4Tile<LPR>::kHeads && h < p.Hkv)
-        *(uint4*)(p.vc + p.tile0(lead / 16, h) + (size_t)i * 16) = *(const uint4*)(tile.v[hl] + i * 16);
+    // (The two tiles are neighbours in the pool.)
+    for (int i = threadIdx.x; i < Int4Tile<LPR>::kHeads * (D + 4); i += 256) {
+        const int hl = i / (D + 4), j = i % (D + 4), h = hg * Int4Tile<LPR>::kHeads + hl;
+        if (h >= p.Hkv) break;
+        if (j < D) *(uint4*)(p.kc + p.tile0(lead / 16, h) + (size_t)j * 16) = *(const uint4*)(&tile.kv[hl][0][0] + j * 16);
+        else ((uint4*)(p.words + p.word(lead / 16, h, 0)))[j - D] = ((const uint4*)tile.words[hl])[j - D];
+    }
 }
 #endif
 

@@ -25,20 +25,24 @@ __global__ void __launch_bounds__(256) append_int4_rows_kernel(Int4View p, const
 // Sixteen rows of one head (or of 16 / LPR heads) per 256-thread workgroup: int4_tile.h.
 template <gg_dtype_t SRC, int LPR>
 __global__ void __launch_bounds__(256) append_int4_tile_kernel(Int4View p, const void* k, const void* v, const int32_t* slots,
-                                                               int n_rows) {
+                                                               int n_rows, unsigned hg) {
     __shared__ Int4Tile<LPR> tile;
     const size_t stride = (size_t)p.Hkv * p.D;
-    int4_tile_rows<LPR>(p, slots, n_rows, blockIdx.x, blockIdx.y, tile, [&](int r, int h, int u, float (&ka)[4], float (&kb)[4], float (&va)[4],
-                                                                           float (&vb)[4], int& oa, int& ob) {
-        const size_t at = (size_t)r * stride + (size_t)h * p.D;
-        oa = 4 * u;
-        ob = p.D / 2 + 4 * u;
-        const auto ra = load4<SRC>(k, at + oa), rb = load4<SRC>(k, at + ob), sa = load4<SRC>(v, at + oa), sb = load4<SRC>(v, at + ob);
-        to_f32<SRC>(ra, ka);
-        to_f32<SRC>(rb, kb);
-        to_f32<SRC>(sa, va);
-        to_f32<SRC>(sb, vb);
-    });
+    int4_tile_rows<SRC, LPR>(
+        p, slots, n_rows, blockIdx.x / hg, blockIdx.x % hg, tile,
+        [&](int r, int h, int u) {
+            const size_t at = (size_t)r * stride + (size_t)h * p.D;
+            const int oa = 4 * u, ob = p.D / 2 + 4 * u;
+            return Int4Raw<SRC>{load4<SRC>(k, at + oa), load4<SRC>(k, at + ob), load4<SRC>(v, at + oa), load4<SRC>(v, at + ob)};
+        },
+        [&](const Int4Raw<SRC>& w, int, int, int u, float (&ka)[4], float (&kb)[4], float (&va)[4], float (&vb)[4], int& oa, int& ob) {
+            oa = 4 * u;
+            ob = p.D / 2 + 4 * u;
+            to_f32<SRC>(w.ka, ka);
+            to_f32<SRC>(w.kb, kb);
+            to_f32<SRC>(w.va, va);
+            to_f32<SRC>(w.vb, vb);
+        });
 }
 
 // A 4-bit pool's rows back, sixteen of one head per workgroup of 2 * head_dim threads: thread (row,
@@ -48,13 +52,13 @@ template <gg_dtype_t DST, int D>
 __global__ void __launch_bounds__(2 * D) read_int4_tile_kernel(Int4View p, void* k_out, void* v_out, const int32_t* slots, int n_rows) {
     constexpr int kC = D / 8;
     __shared__ uint32_t s_v[D / 2 * 4 + D / 16];  // run i at word 4 i + i / 8 (eight runs apart: other banks)
-    const int h = blockIdx.y, row = threadIdx.x / kC, c = threadIdx.x % kC;
+    const int h = blockIdx.x % p.Hkv, group = blockIdx.x / p.Hkv, row = threadIdx.x / kC, c = threadIdx.x % kC;
     const int first = slots[0] < 0 ? 0 : slots[0] % p.bs;  // a prompt's groups start where its blocks do
-    const int r = (int)blockIdx.x * 16 - first % 16 + row;
+    const int r = group * 16 - first % 16 + row;
     const int slot = r >= 0 && r < n_rows ? slots[r] : -1;
     const bool live = slot >= 0 && slot < p.num_slots;
     const int blk = live ? slot / p.bs : 0, off = live ? slot % p.bs : 0;
-    const int lead = slots[min(max((int)blockIdx.x * 16 - first % 16, 0), n_rows - 1)];
+    const int lead = slots[min(max(group * 16 - first % 16, 0), n_rows - 1)];
     const bool whole = __syncthreads_and(live && p.bs == 16 && slot == lead + row && lead % 16 == 0) != 0;
     const uint8_t* vt = p.vc + p.tile0(blk, h);
     if (whole && v_out) {
@@ -123,10 +127,11 @@ gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* 
     if ((p.D == 64 || p.D == 128 || p.D == 256) && (uintptr_t)k % align == 0 && (uintptr_t)v % align == 0) {
         with_float(src, [&](auto t) {
             constexpr gg_dtype_t T = decltype(t)::value;
-            const dim3 grid(int4_tile_groups(n_rows), int4_tile_heads(p.Hkv, p.D));
-            if (p.D == 64) append_int4_tile_kernel<T, 8><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
-            else if (p.D == 128) append_int4_tile_kernel<T, 16><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
-            else append_int4_tile_kernel<T, 32><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows);
+            const unsigned hg = int4_tile_heads(p.Hkv, p.D);
+            const unsigned grid = int4_tile_groups(n_rows) * hg;
+            if (p.D == 64) append_int4_tile_kernel<T, 8><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
+            else if (p.D == 128) append_int4_tile_kernel<T, 16><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
+            else append_int4_tile_kernel<T, 32><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
         });
         return check_hip(hipGetLastError(), "kv_append launch");
     }
@@ -138,9 +143,9 @@ gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* 
 gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype_t dst, const int32_t* slots, int n_rows,
                            hipStream_t s) {
     if (kv->dtype == GG_DTYPE_INT4 && (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) &&
-        (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0 && kv->num_kv_heads <= 65535) {
+        (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0) {
         const Int4View p = int4_view(kv, layer);
-        const dim3 grid(int4_tile_groups(n_rows), p.Hkv);
+        const unsigned grid = int4_tile_groups(n_rows) * p.Hkv;
         with_float(dst, [&](auto t) {
             constexpr gg_dtype_t T = decltype(t)::value;
             if (p.D == 64) read_int4_tile_kernel<T, 64><<<grid, 128, 0, s>>>(p, k_out, v_out, slots, n_rows);

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(RopeArgs a, int heads
 // sixteen rows of a kv head (or two) each, as gg_kv_append does (int4_tile.h).
 template <gg_dtype_t T, int LPR>
 __global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4View p, int q_blocks, int parts, int per,
-                                                                int groups) {
+                                                                int hg) {
     __shared__ Int4Tile<LPR> tile;
     if ((int)blockIdx.x < q_blocks) {
         const unsigned i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -328,21 +328,24 @@ __global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4
     float wa[4], wb[4];
     const Unit x = unit_of(a, threadIdx.x % LPR);
     if (a.k_weight) weight_runs<T>(a.k_weight, x, wa, wb);
-    int4_tile_rows<LPR>(p, a.slots, a.n, b % groups, b / groups, tile,
-                        [&](int t, int h, int u, float (&ka)[4], float (&kb)[4], float (&va)[4], float (&vb)[4], int& oa, int& ob) {
-                            const size_t at = (size_t)t * a.k_stride + (size_t)h * a.D, vat = (size_t)t * a.v_stride + (size_t)h * a.D;
-                            const auto ra = load4<T>(a.k, at + x.oa), rb = load4<T>(a.k, at + x.ob);
-                            const auto sa = load4<T>(a.v, vat + 4 * u), sb = load4<T>(a.v, vat + a.D / 2 + 4 * u);
-                            const Turn r = turn4(a, x, u, t);
-                            to_f32<T>(ra, ka);
-                            to_f32<T>(rb, kb);
-                            to_f32<T>(sa, va);
-                            to_f32<T>(sb, vb);
-                            norm_runs<LPR>(a, a.k_weight != nullptr, wa, wb, ka, kb);
-                            apply_turn(a, x, r, ka, kb);
-                            oa = x.oa;
-                            ob = x.ob;
-                        });
+    int4_tile_rows<T, LPR>(
+        p, a.slots, a.n, b / hg, b % hg, tile,
+        [&](int t, int h, int u) {
+            const size_t at = (size_t)t * a.k_stride + (size_t)h * a.D, vat = (size_t)t * a.v_stride + (size_t)h * a.D;
+            return Int4Raw<T>{load4<T>(a.k, at + x.oa), load4<T>(a.k, at + x.ob), load4<T>(a.v, vat + 4 * u),
+                              load4<T>(a.v, vat + a.D / 2 + 4 * u)};
+        },
+        [&](const Int4Raw<T>& w, int t, int, int u, float (&ka)[4], float (&kb)[4], float (&va)[4], float (&vb)[4], int& oa, int& ob) {
+            const Turn r = turn4(a, x, u, t);
+            to_f32<T>(w.ka, ka);
+            to_f32<T>(w.kb, kb);
+            to_f32<T>(w.va, va);
+            to_f32<T>(w.vb, vb);
+            norm_runs<LPR>(a, a.k_weight != nullptr, wa, wb, ka, kb);
+            apply_turn(a, x, r, ka, kb);
+            oa = x.oa;
+            ob = x.ob;
+        });
 }
 
 // Into the other pools: queries as above, keys and values a row and head a wave.
@@ -390,7 +393,7 @@ gg_status_t launch_vectors(const RopeArgs& a, const KV* kv, const PoolOut& p, hi
     if (all > 0x3fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
     const int some = parts > 0 ? parts : 1;
     if (!kv) qk_norm_rope_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, heads, some, per);
-    else if (tiles) qk_norm_rope_int4_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p.i4, (int)blocks, some, per, (int)groups);
+    else if (tiles) qk_norm_rope_int4_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p.i4, (int)blocks, some, per, (int)int4_tile_heads(a.Hkv, a.D));
     else qk_norm_rope_pool_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p, (int)blocks, some, per);
     return check_hip(hipGetLastError(), "qk_norm_rope launch");
 }
