@@ -45,10 +45,26 @@ __device__ __forceinline__ Int4Scale int4_scale(float lo, float hi) {
     return p;
 }
 
-// (x: int4_clean, within the row's extremes, so that rint(x / s) + z is 0 at least and 16 at most.)
+// (x: int4_clean, within the row's extremes, so that rint(x / s) + z is 0 at least and 16 at most. Adding
+// 1.5 * 2^23 rounds a quotient below 2^22 to a whole number, ties to even, and leaves it in the low bits.)
 __device__ __forceinline__ uint32_t int4_code(float x, const Int4Scale& p) {
-    return (uint32_t)(int)fminf(__builtin_rintf(int4_div(x, p)) + p.z, 15.f);
+    const uint32_t n = __float_as_uint(int4_div(x, p) + 12582912.0f);
+    return min(n + ((uint32_t)(int)p.z - 0x4b400000u), 15u);
 }
+
+// The extremes of a row by whole-number maxima: positive floats order as signed integers and are
+// above all negative ones, negative floats order as unsigned integers and are above all positive ones.
+// (fminf and fmaxf quiet each operand first, and are not merged with the lane exchanges.) A NaN or a
+// value past 1e36 comes out past its bound: `replaced`.
+struct Int4Extremes {
+    int hi = 0;                    // 0.0
+    uint32_t lo = 0x80000000u;     // -0.0
+    __device__ __forceinline__ void take(float a, float b) {
+        hi = max(hi, max((int)__float_as_uint(a), (int)__float_as_uint(b)));
+        lo = max(lo, max(__float_as_uint(a), __float_as_uint(b)));
+    }
+    __device__ __forceinline__ bool replaced() const { return hi > 0x7b4097ce || lo > 0xfb4097ceu; }  // 1e36f, -1e36f
+};
 
 // A token's word: K in the low half, V in the high half.
 __device__ __forceinline__ float int4_k_scale(uint32_t w) { return __uint_as_float((w & 0xfff0u) << 15); }

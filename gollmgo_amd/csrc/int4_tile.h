@@ -91,32 +91,23 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
             float ka[4], kb[4], va[4], vb[4];
             int oa, ob;
             make(raw[round], r, h, u, ka, kb, va, vb, oa, ob);
-            float klo, khi, vlo, vhi;
+            Int4Extremes kx, vx;
             auto extremes = [&] {
-                klo = khi = vlo = vhi = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    klo = fminf(klo, fminf(ka[e], kb[e]));
-                    khi = fmaxf(khi, fmaxf(ka[e], kb[e]));
-                    vlo = fminf(vlo, fminf(va[e], vb[e]));
-                    vhi = fmaxf(vhi, fmaxf(va[e], vb[e]));
-                }
+                kx = vx = Int4Extremes{};
+                kx.take(ka[0], ka[1]), kx.take(ka[2], ka[3]), kx.take(kb[0], kb[1]), kx.take(kb[2], kb[3]);
+                vx.take(va[0], va[1]), vx.take(va[2], va[3]), vx.take(vb[0], vb[1]), vx.take(vb[2], vb[3]);
             };
             extremes();
-            // Values that the rule replaces (NaN, past 1e36) are looked for once per lane: a product with
-            // zero that is not zero, or an extreme past the end.
-            float odd = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                odd = __builtin_fmaf(ka[e], 0.f, __builtin_fmaf(kb[e], 0.f, __builtin_fmaf(va[e], 0.f, __builtin_fmaf(vb[e], 0.f, odd))));
-            if (__builtin_expect(__any(odd != 0.f || fmaxf(khi, vhi) > 1e36f || fminf(klo, vlo) < -1e36f), 0)) {
+            if (__builtin_expect(__any(kx.replaced() || vx.replaced()), 0)) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     ka[e] = int4_clean(ka[e]), kb[e] = int4_clean(kb[e]), va[e] = int4_clean(va[e]), vb[e] = int4_clean(vb[e]);
                 extremes();
             }
-            const Int4Scale ks = int4_scale(group_min<LPR>(klo), group_max<LPR>(khi));
-            const Int4Scale vs = int4_scale(group_min<LPR>(vlo), group_max<LPR>(vhi));
+            auto scale = [](const Int4Extremes& x) {
+                return int4_scale(__uint_as_float(group_max_int<LPR>(x.lo)), __uint_as_float((uint32_t)group_max_int<LPR>(x.hi)));
+            };
+            const Int4Scale ks = scale(kx), vs = scale(vx);
             const int blk = slot / p.bs, off = slot % p.bs;
             const uint32_t k01 = int4_codes4(ka, ks), k23 = int4_codes4(kb, ks), word = ks.half | (vs.half << 16);
             uint32_t vb4[4];

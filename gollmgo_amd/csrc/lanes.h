@@ -5,16 +5,16 @@
 #ifdef __HIPCC__
 namespace gg {
 
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+template <int CTRL, class V>
+__device__ __forceinline__ V dpp(V v) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
 
 // N = 8, 16 or 32 lanes. Steps 1 and 2 exchange within a quad; then a mirror of eight and one of
 // sixteen lanes, where the halves already agree, stand for the exchanges by 4 and 8: all of it in the
 // vector unit (a shuffle is a trip through LDS).
-template <int N, class F>
-__device__ __forceinline__ float group_reduce(float v, F f) {
+template <int N, class V, class F>
+__device__ __forceinline__ V group_reduce(V v, F f) {
     static_assert(N == 8 || N == 16 || N == 32, "group size");
     v = f(v, dpp<0xb1>(v));   // quad_perm [1, 0, 3, 2]
     v = f(v, dpp<0x4e>(v));   // quad_perm [2, 3, 0, 1]
@@ -28,12 +28,13 @@ __device__ __forceinline__ float group_sum(float v) {
     return group_reduce<N>(v, [](float a, float b) { return a + b; });
 }
 template <int N>
-__device__ __forceinline__ float group_min(float v) {
-    return group_reduce<N>(v, [](float a, float b) { return fminf(a, b); });
-}
-template <int N>
 __device__ __forceinline__ float group_max(float v) {
     return group_reduce<N>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+template <int N, class V>
+__device__ __forceinline__ V group_max_int(V v) {
+    return group_reduce<N>(v, [](V a, V b) { return max(a, b); });
 }
 
 // Four consecutive elements of a float type, and back.
