@@ -74,8 +74,8 @@ SIGNATURES = {
     "gg_kv_layer_bytes": (_sz, [_vp]),
     "gg_kv_set_head_scales": (_i, [_vp, _i, C.POINTER(_f), C.POINTER(_f)]),
     "gg_kv_append": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
-    "gg_qk_norm_rope": (_i, [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
-    "gg_qk_norm_rope_append": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _i, _i,
+    "gg_qk_norm_rope": (_i, [_vp, _ll, _vp, _ll, _i, _i, _i, _i, _i, _vp, _vp, _f, _vp, _i, C.c_char_p, _vp, _i, _i, _vp, _vp, _vp]),
+    "gg_qk_norm_rope_append": (_i, [_vp, _i, _vp, _ll, _vp, _ll, _vp, _ll, _i, _i, _i, _vp, _vp, _f, _vp, _i, C.c_char_p, _vp, _i, _i,
                                     _vp, _vp, _vp]),
     "gg_kv_read": (_i, [_vp, _i, _vp, _vp, _i, _vp, _i, _vp]),
     "gg_kv_snapshot_bytes": (_sz, [_vp, _i]),

@@ -55,51 +55,71 @@ def _dev(t: torch.Tensor, name: str, dtype=None) -> int:
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, head_dim: Optional[int] = None):
+def _rows(t: torch.Tensor, name: str):
     """Pointer and row stride of [n_rows, heads, head_dim] rows whose heads are contiguous (a
     slice of a fused projection, or a whole tensor)."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
-    if t.dim() != 3 or (head_dim is not None and t.shape[2] != head_dim):
-        raise ValueError(f"{name} must be [n_rows, heads, head_dim]")
     n, h, d = t.shape
-    if (d > 1 and t.stride(2) != 1) or (h > 1 and t.stride(1) != d):
+    sn, sh, sd = t.stride()
+    if (d > 1 and sd != 1) or (h > 1 and sh != d):
         raise ValueError(f"{name}: the heads of a row must be contiguous")
-    return t.data_ptr(), t.stride(0) if n > 1 else h * d
+    return t.data_ptr(), sn if n > 1 else h * d
+
+
+_STYLES = {"halves": int(RopeStyle.HALVES), "pairs": int(RopeStyle.PAIRS)}
 
 
 def _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style):
-    """The arguments that qk_norm_rope and norm_rope_append share, checked."""
+    """What qk_norm_rope and norm_rope_append share, checked: dtype code, rows, head_dim, and the C
+    arguments from the weights' pointers on: (weights, (positions, axes, pair_axis, inv_freq,
+    pairs, style))."""
     some = q if q is not None else k
     if some is None:
         raise ValueError("q or k is needed")
+    if some.dim() != 3 or (k is not None and k.dim() != 3):
+        raise ValueError("q and k must be [n_rows, heads, head_dim]")
     n, _, d = some.shape
-    if k is not None and (k.dim() != 3 or k.shape[0] != n or k.shape[2] != d or k.dtype != some.dtype):
-        raise ValueError("q and k must share rows, head_dim and dtype")
-    pairs = inv_freq.numel()
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    if positions.dim() != 2 or positions.shape[1] != n:
+    dtype = some.dtype
+    if k is not None and k is not some:
+        kn, _, kd = k.shape
+        if kn != n or kd != d or k.dtype != dtype:
+            raise ValueError("q and k must share rows, head_dim and dtype")
+    shape = positions.shape
+    axes = 1 if len(shape) == 1 else shape[0]
+    if len(shape) > 2 or not len(shape) or shape[-1] != n:
         raise ValueError("positions must be [n_rows] or [axes, n_rows]")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None and (w.shape != (d,) or w.dtype != some.dtype):
-            raise ValueError(f"{name} must be [head_dim] of the rows' dtype")
-    axis = None
+    pairs = inv_freq.numel()
+    wq = wk = axis = None
+    if q_weight is not None:
+        if q_weight.shape != (d,) or q_weight.dtype != dtype:
+            raise ValueError("q_weight must be [head_dim] of the rows' dtype")
+        wq = _dev(q_weight, "q_weight")
+    if k_weight is not None:
+        if k_weight.shape != (d,) or k_weight.dtype != dtype:
+            raise ValueError("k_weight must be [head_dim] of the rows' dtype")
+        wk = _dev(k_weight, "k_weight")
     if pair_axis is not None:
-        if len(pair_axis) != pairs:
-            raise ValueError("pair_axis must name an axis for each of inv_freq's pairs")
-        if any(not 0 <= int(x) < positions.shape[0] for x in pair_axis):
-            raise ValueError("pair_axis names an axis that positions does not have")
-        axis = (C.c_uint8 * max(pairs, 1))(*[int(x) for x in pair_axis])
-    elif positions.shape[0] != 1:
+        axis = bytes(pair_axis)  # (ValueError for what is no small whole number)
+        if len(axis) != pairs or (pairs and max(axis) >= axes):
+            raise ValueError("pair_axis must name an axis of positions for each of inv_freq's pairs")
+    elif axes != 1:
         raise ValueError("several position axes need pair_axis")
-    try:
-        st = RopeStyle[style.upper()]
-    except KeyError as e:
-        raise ValueError(f"unknown style {style!r} (halves, pairs)") from e
-    weights = [_dev(w, "weight") if w is not None else None for w in (q_weight, k_weight)]
-    return n, d, pairs, _dev(positions, "positions", torch.int32), positions.shape[0], axis, _dev(
-        inv_freq, "inv_freq", torch.float32), int(st), weights
+    st = _STYLES.get(style)
+    if st is None:
+        raise ValueError(f"unknown style {style!r} (halves, pairs)")
+    if dtype not in _TORCH_TO_DT:
+        raise TypeError(f"unsupported tensor dtype {dtype}")
+    return int(_TORCH_TO_DT[dtype]), n, d, wq, wk, (_dev(positions, "positions", torch.int32), axes, axis,
+                                                    _dev(inv_freq, "inv_freq", torch.float32), pairs, st)
+
+
+def _out_rows(x: torch.Tensor, out: Optional[torch.Tensor], name: str) -> torch.Tensor:
+    if out is None:
+        return x.new_empty(x.shape)
+    if out.numel() != x.numel() or out.dtype != x.dtype:
+        raise ValueError(f"{name} must be like its input")
+    return out
 
 
 def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -109,24 +129,24 @@ def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions
     """Norm of each head (where its weight is given) and rotation of the first 2 * len(inv_freq)
     dims by positions * inv_freq (gg_qk_norm_rope). q [n, Hq, D], k [n, Hkv, D]: rows may be
     strided (slices of a fused projection); either may be None. positions int32 [n], or
-    [axes, n] with pair_axis naming the axis of each pair. style "halves": dim j with
-    j + pairs; "pairs": 2j with 2j + 1. -> (q_out, k_out), contiguous; q_out may be q itself
-    where that is contiguous."""
-    n, d, pairs, pos, axes, axis, freq, st, (wq, wk) = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style)
-    sides = []
-    for x, o, name in ((q, q_out, "q"), (k, k_out, "k")):
-        if x is None:
-            sides.append((None, 0, 0, None, None))
-            continue
-        ptr, stride = _rows(x, name)
-        if o is None:
-            o = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif o.numel() != x.numel() or o.dtype != x.dtype:
-            raise ValueError(f"{name}_out must be like {name}")
-        sides.append((ptr, stride, x.shape[1], _dev(o, f"{name}_out"), o))
-    (qp, qs, hq, qo, q_out), (kp, ks, hk, ko, k_out) = sides
-    check(lib().gg_qk_norm_rope(qp, qs, kp, ks, int(dtype_of(q if q is not None else k)), n, hq, hk, d, wq, wk, float(eps), pos,
-                                axes, axis, freq, pairs, st, qo, ko, _stream(stream)), "gg_qk_norm_rope")
+    [axes, n] with pair_axis naming the axis of each pair (whole numbers, or bytes). style
+    "halves": dim j with j + pairs; "pairs": 2j with 2j + 1. -> (q_out, k_out), contiguous;
+    q_out may be q itself where that is contiguous."""
+    dt, n, d, wq, wk, rest = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style)
+    qp = kp = qo = ko = None
+    qs = ks = hq = hk = 0
+    if q is not None:
+        qp, qs = _rows(q, "q")
+        hq = q.shape[1]
+        q_out = _out_rows(q, q_out, "q_out")
+        qo = _dev(q_out, "q_out")
+    if k is not None:
+        kp, ks = _rows(k, "k")
+        hk = k.shape[1]
+        k_out = _out_rows(k, k_out, "k_out")
+        ko = _dev(k_out, "k_out")
+    check(lib().gg_qk_norm_rope(qp, qs, kp, ks, dt, n, hq, hk, d, wq, wk, eps, *rest, qo, ko, _stream(stream)),
+          "gg_qk_norm_rope")
     return q_out, k_out
 
 
@@ -240,25 +260,21 @@ class KVCache:
                          q_out: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None):
         """qk_norm_rope with the keys, and the values v [n, Hkv, D] beside them, written to the slots
         of slot_mapping (gg_qk_norm_rope_append; not for INT8 pools) -> q_out."""
-        n, d, pairs, pos, axes, axis, freq, st, (wq, wk) = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis,
-                                                                 style)
-        if k.shape[1:] != (self.num_kv_heads, self.head_dim) or v.shape != k.shape or v.dtype != k.dtype:
+        dt, n, _, wq, wk, rest = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style)
+        if k.shape[1] != self.num_kv_heads or k.shape[2] != self.head_dim or v.shape != k.shape or v.dtype != k.dtype:
             raise ValueError("k and v must be [n_rows, num_kv_heads, head_dim] of one dtype")
         if slot_mapping.numel() != n:
             raise ValueError("slot_mapping must be [n_rows]")
         kp, ks = _rows(k, "k")
         vp, vs = _rows(v, "v")
-        qp, qs, hq, qo = None, 0, 0, None
+        qp = qo = None
+        qs = hq = 0
         if q is not None:
             qp, qs = _rows(q, "q")
             hq = q.shape[1]
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif q_out.numel() != q.numel() or q_out.dtype != q.dtype:
-                raise ValueError("q_out must be like q")
+            q_out = _out_rows(q, q_out, "q_out")
             qo = _dev(q_out, "q_out")
-        check(lib().gg_qk_norm_rope_append(self.handle, layer, qp, qs, kp, ks, vp, vs, int(dtype_of(k)), n, hq, wq, wk, float(eps),
-                                           pos, axes, axis, freq, pairs, st, qo,
+        check(lib().gg_qk_norm_rope_append(self.handle, layer, qp, qs, kp, ks, vp, vs, dt, n, hq, wq, wk, eps, *rest, qo,
                                            _dev(slot_mapping, "slot_mapping", torch.int32), _stream(stream)),
               "gg_qk_norm_rope_append")
         return q_out
@@ -269,19 +285,28 @@ class KVCache:
         [n_rows, num_kv_heads, head_dim] of `dtype` (bfloat16 unless given), or written to
         out = (k, v), of which one may be None. Rows whose slot is negative or past the pool
         are left as they were (in new tensors: not set)."""
-        n = int(slot_mapping.numel())
+        n = slot_mapping.numel()
         if out is None:
-            k, v = (torch.empty(n, self.num_kv_heads, self.head_dim, dtype=dtype or torch.bfloat16,
-                                device=slot_mapping.device) for _ in range(2))
+            k = torch.empty((n, self.num_kv_heads, self.head_dim), dtype=dtype or torch.bfloat16, device=slot_mapping.device)
+            v = torch.empty_like(k)
         else:
             k, v = out
-        given = [t for t in (k, v) if t is not None]
-        if not given or any(t.numel() != n * self.num_kv_heads * self.head_dim for t in given):
-            raise ValueError("k/v must be [n_rows, num_kv_heads, head_dim] matching slot_mapping")
-        if any(t.dtype != given[0].dtype or (dtype is not None and t.dtype != dtype) for t in given):
-            raise TypeError("k and v must share one dtype")
-        check(lib().gg_kv_read(self.handle, layer, _dev(k, "k") if k is not None else None,
-                               _dev(v, "v") if v is not None else None, int(dtype_of(given[0])),
+        kind, ptrs = None, []
+        for t, name in ((k, "k"), (v, "v")):
+            if t is None:
+                ptrs.append(None)
+                continue
+            if t.numel() != n * self.num_kv_heads * self.head_dim:
+                raise ValueError("k/v must be [n_rows, num_kv_heads, head_dim] matching slot_mapping")
+            if kind is not None and t.dtype != kind or dtype is not None and t.dtype != dtype:
+                raise TypeError("k and v must share one dtype")
+            kind = t.dtype
+            ptrs.append(_dev(t, name))
+        if kind is None:
+            raise ValueError("k or v is needed")
+        if kind not in _TORCH_TO_DT:
+            raise TypeError(f"unsupported tensor dtype {kind}")
+        check(lib().gg_kv_read(self.handle, layer, ptrs[0], ptrs[1], int(_TORCH_TO_DT[kind]),
                                _dev(slot_mapping, "slot_mapping", torch.int32), n, _stream(stream)), "gg_kv_read")
         return k, v
 

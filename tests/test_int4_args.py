@@ -56,7 +56,7 @@ def rope_call(**kw):
     (dict(pairs=-1), "num_pairs"), (dict(axes=0), "num_axes"), (dict(axes=9), "num_axes"), (dict(style=2), "style"),
     (dict(eps=float("nan")), "eps"), (dict(eps=-1e-9), "eps"), (dict(qs=255), "overlap"), (dict(ks=127), "overlap"),
     (dict(q=None), "NULL"), (dict(qo=None), "NULL"), (dict(k=None), "NULL"), (dict(ko=None), "NULL"), (dict(pos=None), "NULL"),
-    (dict(freq=None), "NULL"), (dict(axis=(C.c_uint8 * 32)(*[1] * 32)), "pair_axis"),
+    (dict(freq=None), "NULL"), (dict(axis=bytes([1] * 32)), "pair_axis"),
 ])
 def test_norm_rope_refuses_before_any_device_call(bad, word):
     assert rope_call(**bad) == Status.ERR_INVALID
