@@ -63,12 +63,13 @@ __global__ void __launch_bounds__(kFused ? 64 * kFuseParts : 64) attn_generic_ke
     constexpr int kW = kFused ? kFuseParts : 1;
     __shared__ float s_q[64 * DC];
     __shared__ __align__(16) float s_p[kW][64];
-    __shared__ size_t s_vrow[kVRun ? 1 : kW][kVRun ? 1 : 64];
+    constexpr bool kRowsInLds = !kVRun || DT == GG_DTYPE_INT4;  // (V offsets, or 4-bit zero points)
+    __shared__ size_t s_vrow[kRowsInLds ? kW : 1][kRowsInLds ? 64 : 1];
     const size_t qbase = ((size_t)z * a.num_q_heads + h) * D;
     for (int d = threadIdx.x; d < D; d += blockDim.x) s_q[d] = load_as_f32(a.q, a.q_dtype, qbase + d);
     __syncthreads();
     float acc[DC], m, l;
-    generic_partition<DT, DC, kVRun>(a, kv, b, kvh, t0, part < nparts ? t1 : t0, s_q, s_p[wave], s_vrow[kVRun ? 0 : wave],
+    generic_partition<DT, DC, kVRun>(a, kv, b, kvh, t0, part < nparts ? t1 : t0, s_q, s_p[wave], s_vrow[kRowsInLds ? wave : 0],
                                      acc, m, l);
     if constexpr (kFused) {
         __shared__ float s_acc[kFuseParts][64 * DC];
@@ -300,7 +301,9 @@ gg_status_t launch_verify_attention(const AttnArgs& a, hipStream_t s) {
         // V by 16-byte runs: a block is whole runs, a tile of 64 keys whole blocks, and a lane's
         // runs of a tile fit its registers. Every partition of a row in one workgroup: few
         // partitions, few enough dims for the LDS they meet in.
-        const bool vrun = kv->block_size * dtype_bytes(kv->dtype) % 16 == 0 && 64 % kv->block_size == 0 && DC <= 2;
+        // (A 4-bit V run: sixteen tokens.)
+        const size_t run = kv->dtype == GG_DTYPE_INT4 ? 1 : dtype_bytes(kv->dtype);
+        const bool vrun = kv->block_size * run % 16 == 0 && 64 % kv->block_size == 0 && DC <= 2;
         const bool fused = m.max_parts <= kFuseParts && DC <= 2;
         const dim3 grid(fused ? 1 : m.max_parts, m.num_q_heads, m.num_seqs * m.rows);
         const int threads = fused ? 64 * m.max_parts : 64;
@@ -308,9 +311,8 @@ gg_status_t launch_verify_attention(const AttnArgs& a, hipStream_t s) {
             constexpr gg_dtype_t DT = decltype(dt_tag)::value;
             auto small = [&](auto dc_tag) {
                 constexpr int N = decltype(dc_tag)::value;
-                constexpr bool kRun = DT != GG_DTYPE_INT4;  // (4-bit V by element)
-                if (vrun && fused) attn_generic_kernel<DT, N, kRun, true><<<grid, threads, 0, s>>>(m, view);
-                else if (vrun) attn_generic_kernel<DT, N, kRun, false><<<grid, threads, 0, s>>>(m, view);
+                if (vrun && fused) attn_generic_kernel<DT, N, true, true><<<grid, threads, 0, s>>>(m, view);
+                else if (vrun) attn_generic_kernel<DT, N, true, false><<<grid, threads, 0, s>>>(m, view);
                 else if (fused) attn_generic_kernel<DT, N, false, true><<<grid, threads, 0, s>>>(m, view);
                 else attn_generic_kernel<DT, N, false, false><<<grid, threads, 0, s>>>(m, view);
             };

@@ -97,7 +97,7 @@ __device__ __forceinline__ void int4_piece_by_rows(const AttnArgs& a, const KVVi
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         float acc[kDC], m, l;
-        generic_partition<GG_DTYPE_INT4, kDC, false>(a, kv, d.b, d.kvh, d.t0, min(d.t_end, d.ctx - d.nrows + j + 1), s_q, s_p,
+        generic_partition<GG_DTYPE_INT4, kDC, true>(a, kv, d.b, d.kvh, d.t0, min(d.t_end, d.ctx - d.nrows + j + 1), s_q, s_p,
                                                      s_vrow, acc, m, l);
         if (d.rec < 0) {
             const float inv = l > 0.f ? 1.0f / l : 0.f;

@@ -54,8 +54,9 @@ struct Pool16 {
 // line per lane and key) and the merge in a launch, 4 x 5 rows of 8 heads over 64-256 fp32 keys
 // took 14.0 + 4.2 µs, now 8.8; per call on one box, four fp32 sequences of 100-700 keys at
 // head_dim 128 64 -> 25 µs, eight bf16 ones at head_dim 96 132 -> 24.
-// 4-bit pools: codes less their token's zero point, its scales on the score and on p (no V runs:
-// a run of a 16-token block is 8 bytes of two dims each).
+// 4-bit pools: codes less their token's zero point, its scales on the score and on p. A V run of sixteen
+// tokens holds two dims; a lane takes its own half of each byte. (V by element: 16 sequences of
+// 1024 keys, four rows of 16 heads at head_dim 96 145 µs, by runs 37.)
 template <gg_dtype_t DT, int DC, bool kVRun>
 __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVView& kv, int b, int kvh, int t0, int t1,
                                                   const float* s_q, float* s_p, size_t* s_vrow, float (&acc)[DC], float& m,
@@ -65,9 +66,9 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
     const int32_t* bt = a.block_tables + (size_t)b * a.max_blocks;
     const uint8_t* vc = kv.vc;
     constexpr bool kInt4 = DT == GG_DTYPE_INT4;
-    static_assert(!(kInt4 && kVRun), "4-bit V by element");
-    constexpr int kN = Pool16<DT>::kN;
-    constexpr int kRuns = 64 / kN;  // 16-byte V runs of a tile per dim
+    constexpr int kN = Pool16<DT>::kN;             // K elements of 16 bytes
+    constexpr int kNV = kInt4 ? 16 : kN;           // tokens of a 16-byte V run
+    constexpr int kRuns = 64 / kNV;  // 16-byte V runs of a tile per dim
     m = -1e30f;
     l = 0.f;
 #pragma unroll
@@ -92,12 +93,13 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
         if constexpr (kVRun) {
 #pragma unroll
             for (int r = 0; r < kRuns; ++r) {
-                const size_t base = ((size_t)__shfl((unsigned)(vrow >> 32), r * kN) << 32) | (unsigned)__shfl((unsigned)vrow, r * kN);
+                const size_t base = ((size_t)__shfl((unsigned)(vrow >> 32), r * kNV) << 32) | (unsigned)__shfl((unsigned)vrow, r * kNV);
 #pragma unroll
                 for (int c = 0; c < DC; ++c) {
                     const int d = min(lane + 64 * c, D - 1);
                     // (A run past the tile reads its key 0's block: not used.)
-                    vr[c][r] = *(const uint4*)(vc + (base + (size_t)d * kv.bs) * dtype_bytes(DT));
+                    if constexpr (kInt4) vr[c][r] = *(const uint4*)(vc + base + (size_t)(d >= D / 2 ? d - D / 2 : d) * kv.bs);
+                    else vr[c][r] = *(const uint4*)(vc + (base + (size_t)d * kv.bs) * dtype_bytes(DT));
                 }
             }
         }
@@ -115,6 +117,13 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
                     Pool16<DT>::decode(((const uint4*)krow)[v], f);
 #pragma unroll
                     for (int e = 0; e < kN; ++e) dot += s_q[v * kN + e] * (kInt4 ? f[e] - kzero : f[e]);
+                }
+            } else if (kInt4 && D % 8 == 0) {
+#pragma unroll 4
+                for (int v = 0; v < D / 8; ++v) {
+                    const uint32_t w = ((const uint32_t*)krow)[v];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot += s_q[8 * v + e] * ((float)((w >> (4 * e)) & 15u) - kzero);
                 }
             } else {
 #pragma unroll 16
@@ -139,7 +148,8 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
         // One wave's own slots: its LDS operations complete in order.
         __builtin_amdgcn_wave_barrier();
         s_p[lane] = blk >= 0 ? p * (kInt4 ? int4_v_scale(word) : kv.v_scale(blk, kvh)) : 0.f;
-        if constexpr (kInt4) s_vrow[lane] = vrow | ((size_t)int4_v_zero(word) << 60);  // (pools are far below 2^60 bytes)
+        if constexpr (kInt4 && kVRun) ((float*)s_vrow)[lane] = (float)int4_v_zero(word);
+        else if constexpr (kInt4) s_vrow[lane] = vrow | ((size_t)int4_v_zero(word) << 60);  // (pools are far below 2^60 bytes)
         else if constexpr (!kVRun) s_vrow[lane] = vrow;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -147,16 +157,28 @@ __device__ __forceinline__ void generic_partition(const AttnArgs& a, const KVVie
         if constexpr (kVRun) {
 #pragma unroll
             for (int r = 0; r < kRuns; ++r) {
-                if (r * kN >= ntile) break;
-                float pi[kN];
+                if (r * kNV >= ntile) break;
+                float pi[kNV];
 #pragma unroll
-                for (int e = 0; e < kN; ++e) pi[e] = s_p[r * kN + e];
+                for (int e = 0; e < kNV; ++e) pi[e] = s_p[r * kNV + e];
+                if constexpr (kInt4) {
+                    // (Codes are finite: masked and skipped keys have p = 0.)
 #pragma unroll
-                for (int c = 0; c < DC; ++c) {
-                    float f[kN];
-                    Pool16<DT>::decode(vr[c][r], f);
+                    for (int c = 0; c < DC; ++c) {
+                        const uint32_t w[4] = {vr[c][r].x, vr[c][r].y, vr[c][r].z, vr[c][r].w};
+                        const int shift = lane + 64 * c >= D / 2 ? 4 : 0;
 #pragma unroll
-                    for (int e = 0; e < kN; ++e) acc[c] += pi[e] * (r * kN + e < ntile ? f[e] : 0.f);
+                        for (int e = 0; e < kNV; ++e)
+                            acc[c] += pi[e] * ((float)((w[e >> 2] >> (8 * (e & 3) + shift)) & 15u) - ((const float*)s_vrow)[r * kNV + e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < DC; ++c) {
+                        float f[kN];
+                        Pool16<DT>::decode(vr[c][r], f);
+#pragma unroll
+                        for (int e = 0; e < kN; ++e) acc[c] += pi[e] * (r * kN + e < ntile ? f[e] : 0.f);
+                    }
                 }
             }
         } else {

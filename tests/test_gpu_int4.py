@@ -253,6 +253,7 @@ SHAPES = [
     (64, 16, 16, 2, 8, [900, 8, 33], [8, 8, 5]),
     (128, 16, 12, 2, 8, [1100, 9, 31], [8, 7, 1]),
     (80, 16, 4, 2, 3, [3, 100, 700], None),
+    (96, 16, 6, 3, 2, [2, 65, 500], [2, 1, 2]), (128, 32, 4, 2, 2, [2, 70, 300], None), (120, 64, 4, 1, 2, [130, 5], None),
     (128, 8, 4, 2, 2, [2, 70], None),
     (256, 16, 2, 1, 2, [90, 600], None),
     (34, 7, 3, 3, 2, [2, 20], None),
