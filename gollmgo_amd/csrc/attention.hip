@@ -23,6 +23,7 @@
 //     narrow tables and explicit partitions of attention_full.hip's shapes, and for scales that
 //     the MFMA softmax does not take (attn_mfma_scale). Its partitions and the MFMA partition grid
 //     share one partial format and one combine kernel.
+#include <algorithm>
 #include <type_traits>
 
 #include "gg_common.h"
@@ -237,10 +238,22 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
 bool attn_rows_faster(const KV* kv, int num_seqs, int rows, int num_q_heads, int max_blocks, bool plans) {
     const AttnShape sh = attn_shape(kv, rows, num_q_heads);
     const long long keys = (long long)max_blocks * kv->block_size;
-    if (!sh.full || keys > 64 * kFuseParts || kv->dtype == GG_DTYPE_INT4) return false;
+    if (!sh.full || keys > 64 * kFuseParts) return false;
     const bool wide = kv->head_dim == 128, byte = dtype_bytes(kv->dtype) == 1;
     const double k = (double)keys, heads = (double)num_seqs * rows * num_q_heads;
     const double items = (double)num_seqs * kv->num_kv_heads * sh.groups;
+    if (kv->dtype == GG_DTYPE_INT4) {
+        // No plan at these widths (a workgroup per item), and the per-row kernel reads a tile of 64 keys
+        // at the price of one. From 180 shapes (both head_dims, 1 to 512 sequences, 16 to 512 keys,
+        // 1 and 4 query heads per kv head, 1 and 5 rows), in graphs on one box, pieces / rows: 512
+        // sequences of 16 keys, 8 heads, head_dim 128 43.6 / 11.6 µs; 16 of 512, 5 rows of 32 heads 11.7
+        // / 70; one of 64, 5 rows, head_dim 64 8.1 / 4.6.
+        const double rows4 = (wide ? 5.9 : 4.2) + 0.0045 * k +
+                             heads * 1e-3 * (wide ? std::max(1.72 + 0.005 * k, 0.034 * k) : std::max(0.95 + 0.005 * k, 0.0195 * k));
+        const double slope = sh.nt == 1 ? (wide ? 0.0105 : 0.0061) : (wide ? 0.0195 : 0.0148);
+        const double pieces4 = (wide ? 6.2 : 5.7) + (sh.nt - 1) * (wide ? 3.5 : 2.2) + 0.003 * k + std::max(items - 512, 0.0) * slope;
+        return rows4 < pieces4 - (plans ? 0 : 2.5);  // (a planned call's draft rows: a launch of their own)
+    }
     // The latency of one workgroup, and the throughput per query row and head.
     const double by_rows = (wide ? 5.3 + 0.01 * k : 4.5 + 0.005 * k) +
                            heads * 1e-3 * (wide ? 0.8 + (byte ? 0.024 : 0.035) * k : 0.5 + (byte ? 0.018 : 0.02) * k);

@@ -302,13 +302,14 @@ def test_attention_partitions(gv, partition):
     kv.close()
 
 
+@pytest.mark.parametrize("wide", [None, 80])  # (a table past 512 keys: by pieces)
 @pytest.mark.parametrize("d", [64, 128])
-def test_attention_holes_in_the_table(gv, d):
+def test_attention_holes_in_the_table(gv, d, wide):
     """Blocks missing from a table (negative ids, ids past the pool) hide their keys; a row that
     sees no key at all gives zeros."""
     rng = np.random.default_rng(2)
     ctx = [400, 100, 40, 17]
-    kv, tables = filled(gv, rng, ctx, 2, d, 16)
+    kv, tables = filled(gv, rng, ctx, 2, d, 16, wide)
     tables[0, 3], tables[0, 10], tables[0, 24] = -1, kv.num_blocks, -7
     tables[1, :] = -1
     tables[2, 0] = 1 << 20
@@ -318,10 +319,11 @@ def test_attention_holes_in_the_table(gv, d):
     kv.close()
 
 
-def test_attention_no_rows_and_no_keys(gv):
+@pytest.mark.parametrize("wide", [None, 80])
+def test_attention_no_rows_and_no_keys(gv, wide):
     rng = np.random.default_rng(4)
     ctx = [0, -5, 2, 50]
-    kv, tables = filled(gv, rng, [16, 16, 16, 50], 2, 128, 16)
+    kv, tables = filled(gv, rng, [16, 16, 16, 50], 2, 128, 16, wide)
     check_attention(gv, kv, tables, rng, ctx, [2, 2, 3, 0], 3, 4)  # all: nothing to write
     kv.close()
 
@@ -345,14 +347,15 @@ def test_attention_over_other_rows(gv, kind, d):
     kv.close()
 
 
+@pytest.mark.parametrize("wide", [None, 80])
 @pytest.mark.parametrize("odt", ["bf16", "f32"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_attention_value_scales_far_apart(gv, d, odt):
+def test_attention_value_scales_far_apart(gv, d, odt, wide):
     """Tokens whose values differ by 2^60: a token hidden from a row, or nearly unweighted, must
     not cost the others their digits."""
     rng = np.random.default_rng(7)
     ctx, h, R = [200, 70], 2, 4
-    kv, tables = filled(gv, rng, ctx, h, d, 16)
+    kv, tables = filled(gv, rng, ctx, h, d, 16, wide)
     slots = np.concatenate([tables[b, np.arange(c) // 16] * 16 + np.arange(c) % 16 for b, c in enumerate(ctx)]).astype(np.int32)
     k, _ = to_dev(rows_of(rng, sum(ctx), h, d), "bf16")
     v = rows_of(rng, sum(ctx), h, d)
@@ -364,14 +367,15 @@ def test_attention_value_scales_far_apart(gv, d, odt):
     kv.close()
 
 
+@pytest.mark.parametrize("wide", [None, 80])
 @pytest.mark.parametrize("qdt", ["bf16", "f32"])
 @pytest.mark.parametrize("d", [64, 128])
-def test_attention_queries_of_any_size(gv, d, qdt):
+def test_attention_queries_of_any_size(gv, d, qdt, wide):
     """Rows of one item whose sizes lie far apart, a row of zeros, and one with a NaN or an
     infinity: each row as if it were alone."""
     rng = np.random.default_rng(8)
     ctx, R, hq = [150], 4, 4
-    kv, tables = filled(gv, rng, ctx, 1, d, 16)
+    kv, tables = filled(gv, rng, ctx, 1, d, 16, wide)
     q = rng.normal(0, 1, (1, R, hq, d))
     q[0, 0] *= 2.0 ** -60
     q[0, 1] *= 2.0 ** 6
@@ -394,14 +398,15 @@ def test_attention_queries_of_any_size(gv, d, qdt):
 @pytest.mark.parametrize("d,hq,h,R,ctx,rows", [
     (128, 32, 8, 5, [5, 20, 300, 1000, 64], [5, 1, 3, 5, 4]), (128, 8, 1, 9, [9, 900], None), (64, 8, 2, 4, [4, 33, 500], None),
     (128, 16, 2, 12, [700, 12], None), (80, 4, 2, 3, [3, 90], None), (128, 8, 2, 20, [500, 20], None)])
+@pytest.mark.parametrize("wide", [None, 80])
 @pytest.mark.parametrize("src", ["bf16", "f32"])
-def test_append_attention_equals_the_two_calls(gv, d, hq, h, R, ctx, rows, src):
+def test_append_attention_equals_the_two_calls(gv, d, hq, h, R, ctx, rows, src, wide):
     say(f"int4 append+attention d={d} hq={hq} h={h} R={R} {ctx} {src}")
     rng = np.random.default_rng(R)
     B = len(ctx)
     pools = []
     for _ in range(2):
-        pools.append(filled(gv, np.random.default_rng(11), ctx, h, d, 16))
+        pools.append(filled(gv, np.random.default_rng(11), ctx, h, d, 16, wide))
     (kv1, tables), (kv2, _) = pools
     counts = np.asarray(rows if rows is not None else [R] * B, np.int32)
     k, kf = to_dev(rows_of(rng, B * R, h, d, "outliers"), src)
@@ -424,6 +429,35 @@ def test_append_attention_equals_the_two_calls(gv, d, hq, h, R, ctx, rows, src):
     assert torch.equal(o1, o2)
     check_pool(kv1, 0, kf, vf, slots.reshape(-1))
     kv1.close(), kv2.close()
+
+
+@pytest.mark.parametrize("io", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("d,R,hq,h", [(64, 5, 16, 4), (128, 5, 16, 4), (128, 1, 16, 2), (128, 9, 10, 2), (64, 8, 8, 1)])
+def test_attention_whole_items(gv, d, R, hq, h, io):
+    """Tables too narrow to cut and batches too large for the per-row kernel."""
+    rng = np.random.default_rng(R)
+    ctx = rng.integers(R, 350, 70)
+    kv, tables = filled(gv, rng, ctx, h, d, 16)
+    rows = rng.integers(1, R + 1, 70)
+    check_attention(gv, kv, tables, rng, ctx, rows, R, hq, io, io)
+    kv.close()
+
+
+def test_attention_stale_slots(gv):
+    """Rows behind a sequence's end, and in no block of its table, hold values 2^90 times larger: they
+    change nothing."""
+    rng = np.random.default_rng(21)
+    ctx, h, d = [75, 130, 700], 2, 128
+    kv, tables = filled(gv, rng, ctx, h, d, 16)
+    every = np.arange(kv.num_blocks * 16)
+    live = np.concatenate([tables[b, np.arange(c) // 16] * 16 + np.arange(c) % 16 for b, c in enumerate(ctx)])
+    stale = np.setdiff1d(every, live).astype(np.int32)
+    big, _ = to_dev(rows_of(rng, len(stale), h, d) * 2.0 ** 90, "bf16")
+    kv.append(0, big, big, torch.from_numpy(stale).cuda())
+    tables[1, 2] = -1
+    for odt in ("bf16", "f32"):
+        check_attention(gv, kv, tables, rng, ctx, None, 3, 8, "bf16", odt)
+    kv.close()
 
 
 def test_attention_many_sequences(gv):
