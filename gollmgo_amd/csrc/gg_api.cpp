@@ -110,6 +110,8 @@ GG_API gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size, 
     // the paged pattern gains ~4 %, the attention kernel ~0.5 %).
     gg_status_t st = check_hip(hipMalloc((void**)&kv->k_pool, kv->layer_stride * num_layers), "hipMalloc(KV pool)");
     if (st == GG_OK) kv->v_pool = kv->k_pool + kv->tile_bytes;
+    // Slots never written hold zeros, whatever the memory held before.
+    if (st == GG_OK) st = check_hip(hipMemset(kv->k_pool, 0, kv->layer_stride * num_layers), "KV pool init");
     if (st == GG_OK && scale_mode == GG_SCALE_PER_HEAD) {
         kv->scale_layer_elems = (size_t)2 * num_kv_heads;  // scales then inverse scales
         size_t b = kv->scale_layer_elems * num_layers * sizeof(float);
@@ -137,6 +139,8 @@ GG_API gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size, 
         st = check_hip(hipMalloc(&kv->k_scales, b), "hipMalloc(token scales)");
         if (st == GG_OK) st = check_hip(hipMemset(kv->k_scales, 0, b), "scales init");
     }
+    // (The fills run on the null stream; the pool may be used on any other next.)
+    if (st == GG_OK) st = check_hip(hipStreamSynchronize(nullptr), "KV pool init");
     if (st != GG_OK) {
         std::string msg = t_last_error;
         (void)hipFree(kv->k_pool);

@@ -107,7 +107,8 @@ gg_status_t gg_sync(void* stream);
  * Replaces gollmgo_kvcache_create / _k_layer_ptr / _v_layer_ptr / _destroy
  * (kernels/gollmgo_kvcache.h:26-35,66). The reference takes num_slots and stores
  * 2-byte elements only (gollmgo_kvcache.cu:39-40); here the pool is sized in
- * blocks and the element type and scale mode are chosen at creation.
+ * blocks and the element type and scale mode are chosen at creation. Slots that were
+ * never written hold zeros.
  * ------------------------------------------------------------------------- */
 gg_status_t gg_kv_create(int num_layers, int num_blocks, int block_size,
                          int num_kv_heads, int head_dim, gg_dtype_t dtype,
