@@ -196,7 +196,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
     if (kv->dtype == GG_DTYPE_INT4) {
         // A workgroup per item where the plan would cut nothing (tables below the shortest piece) or
         // cannot rank the batch.
-        if (!sh.full || (long long)num_seqs * kv->num_kv_heads * sh.groups > 0x7fffffffLL)
+        if (!sh.full || (long long)num_seqs * kv->num_kv_heads * sh.groups > max_blocks_of(256))
             return {ATTN_SCHED_GRID, attn_generic_partition(kv, num_seqs, rows, num_q_heads, max_blocks)};
         const int tok = int4_chunk_tokens(sh.nt);
         const bool narrow = (long long)max_blocks * kv->block_size <= tok * lpt_min_chunks_of(kv, tok);

@@ -255,6 +255,17 @@ GG_API gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void
     return launch_kv_append(kv, layer, k, v, src_dtype, slot_mapping, n_rows, (hipStream_t)stream);
 }
 
+// A call that reads or writes a pool runs on the pool's own device.
+static gg_status_t on_pool_device(gg_kv_t kv, const char* who) {
+    int dev = 0;
+    const gg_status_t st = check_hip(hipGetDevice(&dev), "hipGetDevice");
+    if (st != GG_OK) return st;
+    if (dev != kv->device)
+        return fail(GG_ERR_INVALID, std::string(who) + ": the pool is on device " + std::to_string(kv->device) +
+                                        ", the current device is " + std::to_string(dev));
+    return GG_OK;
+}
+
 // ---------------------------------------------------------------- norm and rotation
 
 static gg_status_t rope_args(RopeArgs& a, const char* who, const void* q, long long q_stride, const void* k, long long k_stride,
@@ -350,6 +361,8 @@ GG_API gg_status_t gg_qk_norm_rope_append(gg_kv_t kv, int layer, const void* q, 
                  "gg_qk_norm_rope_append: rows overlap (stride below heads * head_dim)");
     if (n_rows == 0) return GG_OK;
     GG_CHECK_ARG(v && slot_mapping, "gg_qk_norm_rope_append: NULL buffer");
+    const gg_status_t dev = on_pool_device(kv, "gg_qk_norm_rope_append");
+    if (dev != GG_OK) return dev;
     a.v = v;
     a.v_stride = v_stride;
     a.slots = slot_mapping;
@@ -365,6 +378,8 @@ GG_API gg_status_t gg_kv_read(gg_kv_t kv, int layer, void* k_out, void* v_out, g
     GG_CHECK_ARG(is_float_io(out_dtype), "gg_kv_read: out dtype must be F32/F16/BF16");
     if (n_rows == 0) return GG_OK;
     GG_CHECK_ARG(slot_mapping && (k_out || v_out), "gg_kv_read: NULL buffer");
+    const gg_status_t dev = on_pool_device(kv, "gg_kv_read");
+    if (dev != GG_OK) return dev;
     return launch_kv_read(kv, layer, k_out, v_out, out_dtype, slot_mapping, n_rows, (hipStream_t)stream);
 }
 

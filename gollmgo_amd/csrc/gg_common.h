@@ -18,6 +18,9 @@ void clear_error();
 gg_status_t fail(gg_status_t st, const std::string& msg);
 gg_status_t check_hip(hipError_t e, const char* what);
 
+// Most workgroups of a launch of `threads` each (a grid holds below 2^32 threads).
+constexpr long long max_blocks_of(int threads) { return 0xffffffffLL / threads; }
+
 // ---- KV cache handle ----
 struct KV {
     int num_layers = 0;

@@ -122,13 +122,16 @@ __global__ void __launch_bounds__(256) read_rows_kernel(KVView kv, void* k_out, 
 gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* v, gg_dtype_t src, const int32_t* slots,
                                   int n_rows, hipStream_t s) {
     const Int4View p = int4_view(kv, layer);
+    const char* too_many = "gg_kv_append: too many rows for one call";
     // By tiles of sixteen rows: head_dims of 8, 16 or 32 lanes of eight dims, vector loads.
     const size_t align = src == GG_DTYPE_F32 ? 16 : 8;
     if ((p.D == 64 || p.D == 128 || p.D == 256) && (uintptr_t)k % align == 0 && (uintptr_t)v % align == 0) {
+        const unsigned hg = int4_tile_heads(p.Hkv, p.D);
+        const long long blocks = (long long)int4_tile_groups(n_rows) * hg;
+        if (blocks > max_blocks_of(256)) return fail(GG_ERR_INVALID, too_many);
+        const unsigned grid = (unsigned)blocks;
         with_float(src, [&](auto t) {
             constexpr gg_dtype_t T = decltype(t)::value;
-            const unsigned hg = int4_tile_heads(p.Hkv, p.D);
-            const unsigned grid = int4_tile_groups(n_rows) * hg;
             if (p.D == 64) append_int4_tile_kernel<T, 8><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
             else if (p.D == 128) append_int4_tile_kernel<T, 16><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
             else append_int4_tile_kernel<T, 32><<<grid, 256, 0, s>>>(p, k, v, slots, n_rows, hg);
@@ -136,6 +139,7 @@ gg_status_t launch_kv_append_int4(KV* kv, int layer, const void* k, const void* 
         return check_hip(hipGetLastError(), "kv_append launch");
     }
     const long long waves = (long long)n_rows * p.Hkv;
+    if ((waves + 3) / 4 > max_blocks_of(256)) return fail(GG_ERR_INVALID, too_many);
     append_int4_rows_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(p, k, v, src, slots, n_rows);
     return check_hip(hipGetLastError(), "kv_append launch");
 }
@@ -145,7 +149,9 @@ gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype
     if (kv->dtype == GG_DTYPE_INT4 && (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) &&
         (uintptr_t)k_out % 16 == 0 && (uintptr_t)v_out % 16 == 0) {
         const Int4View p = int4_view(kv, layer);
-        const unsigned grid = int4_tile_groups(n_rows) * p.Hkv;
+        const long long blocks = (long long)int4_tile_groups(n_rows) * p.Hkv;
+        if (blocks > max_blocks_of(2 * p.D)) return fail(GG_ERR_INVALID, "gg_kv_read: too many rows for one call");
+        const unsigned grid = (unsigned)blocks;
         with_float(dst, [&](auto t) {
             constexpr gg_dtype_t T = decltype(t)::value;
             if (p.D == 64) read_int4_tile_kernel<T, 64><<<grid, 128, 0, s>>>(p, k_out, v_out, slots, n_rows);
@@ -156,7 +162,7 @@ gg_status_t launch_kv_read(KV* kv, int layer, void* k_out, void* v_out, gg_dtype
     }
     const KVView view = make_kv_view(kv, layer);
     const long long n = (long long)n_rows * view.Hkv * view.D;
-    if ((n + 255) / 256 > 0x7fffffffLL) return fail(GG_ERR_INVALID, "gg_kv_read: too many elements for one call");
+    if ((n + 255) / 256 > max_blocks_of(256)) return fail(GG_ERR_INVALID, "gg_kv_read: too many rows for one call");
     read_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(view, k_out, v_out, dst, slots, n_rows);
     return check_hip(hipGetLastError(), "kv_read launch");
 }

@@ -390,7 +390,7 @@ gg_status_t launch_vectors(const RopeArgs& a, const KV* kv, const PoolOut& p, hi
     const long long all = blocks + (!kv     ? 0
                                     : tiles ? (long long)groups * int4_tile_heads(a.Hkv, a.D)
                                             : ((long long)a.n * a.Hkv + 3) / 4);
-    if (all > 0x3fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+    if (all > max_blocks_of(256)) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
     const int some = parts > 0 ? parts : 1;
     if (!kv) qk_norm_rope_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, heads, some, per);
     else if (tiles) qk_norm_rope_int4_kernel<T, LPR><<<(unsigned)all, 256, 0, s>>>(a, p.i4, (int)blocks, some, per, (int)int4_tile_heads(a.Hkv, a.D));
@@ -425,7 +425,7 @@ gg_status_t launch_qk_norm_rope(const RopeArgs& a, KV* kv, int layer, hipStream_
         return st;
     }
     const long long waves = (long long)a.n * (a.Hq + a.Hkv);
-    if ((waves + 3) / 4 > 0x7fffffffLL) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
+    if ((waves + 3) / 4 > max_blocks_of(256)) return fail(GG_ERR_INVALID, "qk_norm_rope: too many rows for one call");
     qk_norm_rope_rows_kernel<<<(unsigned)((waves + 3) / 4), 256, 0, s>>>(a, p);
     return check_hip(hipGetLastError(), "qk_norm_rope launch");
 }

@@ -79,6 +79,8 @@ def _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style):
         raise ValueError("q or k is needed")
     if some.dim() != 3 or (k is not None and k.dim() != 3):
         raise ValueError("q and k must be [n_rows, heads, head_dim]")
+    if some.is_cuda and some.get_device() != torch.cuda.current_device():
+        raise ValueError("the rows are on another device than the current one")
     n, _, d = some.shape
     dtype = some.dtype
     if k is not None and k is not some:

@@ -527,3 +527,35 @@ def test_streams_and_noalloc(gv):
     torch.cuda.synchronize()
     assert torch.equal(a, b) and torch.equal(a, c)
     kv.close()
+
+
+def test_offsets_past_32_bits(gv):
+    """Blocks past 4 GiB of a pool: written, read and attended to as the same rows in a small pool."""
+    say("int4 pool past 4 GiB")
+    rng = np.random.default_rng(31)
+    h, d, nb = 8, 128, 300_000
+    ctx, R, hq = [700, 40, 1300], 3, 16
+    small, tables = filled(gv, rng, ctx, h, d, 16)
+    far = np.where(tables >= 0, nb - 1 - tables, -1).astype(np.int32)
+    big = gv.KVCache(1, nb, 16, h, d, DType.INT4)
+    n = small.num_blocks * 16
+    k, _ = to_dev(rows_of(rng, n, h, d), "bf16")
+    v, _ = to_dev(rows_of(rng, n, h, d), "bf16")
+    slots = np.arange(n, dtype=np.int32)
+    far_slots = ((nb - 1 - slots // 16) * 16 + slots % 16).astype(np.int32)
+    sd, fd = torch.from_numpy(slots).cuda(), torch.from_numpy(far_slots).cuda()
+    for kv, s in ((small, sd), (big, fd)):
+        kv.append(0, k, v, s)
+    for a, b in zip(small.read(0, sd), big.read(0, fd)):
+        assert torch.equal(a, b)
+    q, _ = to_dev(rng.normal(0, 1, (3, R, hq, d)).astype(np.float32), "bf16")
+    cd = torch.tensor(ctx, dtype=torch.int32).cuda()
+    o1, o2 = torch.zeros_like(q), torch.zeros_like(q)
+    small.attention(0, q, o1, cd, torch.from_numpy(tables).cuda(), 0.1)
+    big.attention(0, q, o2, cd, torch.from_numpy(far).cuda(), 0.1)
+    assert torch.equal(o1, o2) and o1.abs().sum() > 0
+    o3, o4 = torch.zeros_like(q), torch.zeros_like(q)  # the per-row kernel
+    small.attention(0, q, o3, cd, torch.from_numpy(tables).cuda(), 0.1, partition_tokens=512)
+    big.attention(0, q, o4, cd, torch.from_numpy(far).cuda(), 0.1, partition_tokens=512)
+    assert torch.equal(o3, o4)
+    small.close(), big.close()

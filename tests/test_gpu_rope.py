@@ -290,3 +290,25 @@ def test_graph_of_a_layer(gv):
         torch.cuda.synchronize()
         assert torch.equal(got, e_o) and e_o.abs().sum() > 0
     kv.close()
+
+
+def test_offsets_past_32_bits(gv):
+    """Rows 2^20 elements apart: the last ones start past 2^32 bytes."""
+    rng = np.random.default_rng(7)
+    n, hq, hk, d = 2500, 4, 2, 128
+    wide = torch.empty(n, 1 << 20, dtype=torch.bfloat16, device="cuda")
+    fused, w, pos, freq, axis = inputs(rng, n, hq, hk, d, "bf16", 64, 1, 5)
+    wide[:, :(hq + 2 * hk) * d] = fused.view(n, -1)
+    x = wide[:, :(hq + 2 * hk) * d].unflatten(1, (hq + 2 * hk, d))
+    kw = dict(positions=torch.from_numpy(pos).cuda(), inv_freq=torch.from_numpy(freq).cuda(), q_weight=w[0], k_weight=w[1])
+    a = gv.qk_norm_rope(fused[:, :hq], fused[:, hq:hq + hk], **kw)
+    b = gv.qk_norm_rope(x[:, :hq], x[:, hq:hq + hk], **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    got = []
+    for src in (fused, x):
+        kv = gv.KVCache(1, n // 16 + 1, 16, hk, d, DType.INT4)
+        kv.norm_rope_append(0, src[:, :hq], src[:, hq:hq + hk], src[:, hq + hk:], slot_mapping=slots, **kw)
+        got.append(kv.read(0, slots))
+        kv.close()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
