@@ -120,6 +120,51 @@ func (c *KVCache) Append(layer int, k, v unsafe.Pointer, slots unsafe.Pointer, n
 		(*C.int32_t)(slots), C.int(n), stream))
 }
 
+// Read returns the rows in n slots of one layer as bf16 numbers: k, v device [n][Hkv][D], either
+// may be nil. Rows of negative slots are left as they were.
+func (c *KVCache) Read(layer int, k, v unsafe.Pointer, slots unsafe.Pointer, n int, stream unsafe.Pointer) error {
+	return ggErr("gg_kv_read", C.gg_kv_read(c.h, C.int(layer), k, v, C.GG_DTYPE_BF16, (*C.int32_t)(slots),
+		C.int(n), stream))
+}
+
+// Rope is what the norm and rotation of a model's rows keep from layer to layer: the frequencies
+// (device float[Pairs]) and the axis of each pair (nil: all of the first).
+type Rope struct {
+	InvFreq  unsafe.Pointer
+	Pairs    int
+	PairAxis []byte
+	Axes     int
+	Style    int
+	Eps      float32
+}
+
+func (r *Rope) axis() *C.uint8_t {
+	if len(r.PairAxis) == 0 {
+		return nil
+	}
+	return (*C.uint8_t)(unsafe.Pointer(&r.PairAxis[0]))
+}
+
+// QKNormRope norms (where a weight is given) and rotates n rows of query and key heads (bf16, rows
+// qStride and kStride elements apart) into dense rows. positions: device int32[r.Axes][n].
+func QKNormRope(r *Rope, q unsafe.Pointer, qStride int, k unsafe.Pointer, kStride, n, Hq, Hkv, D int,
+	qWeight, kWeight, positions, qOut, kOut, stream unsafe.Pointer) error {
+	st := C.gg_qk_norm_rope(q, C.longlong(qStride), k, C.longlong(kStride), C.GG_DTYPE_BF16, C.int(n), C.int(Hq),
+		C.int(Hkv), C.int(D), qWeight, kWeight, C.float(r.Eps), (*C.int32_t)(positions), C.int(r.Axes), r.axis(),
+		(*C.float)(r.InvFreq), C.int(r.Pairs), C.gg_rope_style_t(r.Style), qOut, kOut, stream)
+	return ggErr("gg_qk_norm_rope", st)
+}
+
+// QKNormRopeAppend is QKNormRope with keys and values written to the pool's slots instead.
+func (c *KVCache) QKNormRopeAppend(layer int, r *Rope, q unsafe.Pointer, qStride int, k unsafe.Pointer, kStride int,
+	v unsafe.Pointer, vStride, n, Hq int, qWeight, kWeight, positions, qOut, slots, stream unsafe.Pointer) error {
+	st := C.gg_qk_norm_rope_append(c.h, C.int(layer), q, C.longlong(qStride), k, C.longlong(kStride), v,
+		C.longlong(vStride), C.GG_DTYPE_BF16, C.int(n), C.int(Hq), qWeight, kWeight, C.float(r.Eps),
+		(*C.int32_t)(positions), C.int(r.Axes), r.axis(), (*C.float)(r.InvFreq), C.int(r.Pairs),
+		C.gg_rope_style_t(r.Style), qOut, (*C.int32_t)(slots), stream)
+	return ggErr("gg_qk_norm_rope_append", st)
+}
+
 // Attention runs the verify attention of one layer for B sequences with up to R rows.
 // q/out: device [B][R][Hq][D] bf16; ctxLens, rowCounts: device int32[B];
 // blockTables: device int32[B][maxBlocks]; ws: device workspace of wsBytes.
@@ -256,8 +301,13 @@ const (
 	DtypeBF16 = int(C.GG_DTYPE_BF16)
 	DtypeFP8  = int(C.GG_DTYPE_FP8_E4M3)
 	DtypeINT8 = int(C.GG_DTYPE_INT8)
+	DtypeINT4 = int(C.GG_DTYPE_INT4) // pools only, with ScalePerToken
 
 	ScaleNone     = int(C.GG_SCALE_NONE)
 	ScalePerHead  = int(C.GG_SCALE_PER_HEAD)
 	ScalePerBlock = int(C.GG_SCALE_PER_BLOCK)
+	ScalePerToken = int(C.GG_SCALE_PER_TOKEN)
+
+	RopeHalves = int(C.GG_ROPE_HALVES)
+	RopePairs  = int(C.GG_ROPE_PAIRS)
 )
