@@ -198,7 +198,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
         // cannot rank the batch.
         if (!sh.full || (long long)num_seqs * kv->num_kv_heads * sh.groups > max_blocks_of(256))
             return {ATTN_SCHED_GRID, attn_generic_partition(kv, num_seqs, rows, num_q_heads, max_blocks)};
-        const int tok = int4_chunk_tokens(sh.nt);
+        const int tok = attn_kv_chunk_tokens(kv, sh, num_seqs);
         const bool narrow = (long long)max_blocks * kv->block_size <= tok * lpt_min_chunks_of(kv, tok);
         const bool ranked = num_seqs <= kLptMaxSeqs && (long long)num_seqs * kv->num_kv_heads * sh.groups <= (1 << 18);
         return {narrow || !ranked ? ATTN_SCHED_ITEMS : ATTN_SCHED_LPT, 0};
@@ -246,11 +246,11 @@ bool attn_rows_faster(const KV* kv, int num_seqs, int rows, int num_q_heads, int
         // No plan at these widths (a workgroup per item), and the per-row kernel reads a tile of 64 keys
         // at the price of one. From 180 shapes (both head_dims, 1 to 512 sequences, 16 to 512 keys,
         // 1 and 4 query heads per kv head, 1 and 5 rows), in graphs on one box, pieces / rows: 512
-        // sequences of 16 keys, 8 heads, head_dim 128 43.6 / 11.6 µs; 16 of 512, 5 rows of 32 heads 11.7
+        // sequences of 16 keys, 8 heads, head_dim 128 28 / 11.6 µs; 16 of 512, 5 rows of 32 heads 11.7
         // / 70; one of 64, 5 rows, head_dim 64 8.1 / 4.6.
         const double rows4 = (wide ? 5.9 : 4.2) + 0.0045 * k +
                              heads * 1e-3 * (wide ? std::max(1.72 + 0.005 * k, 0.034 * k) : std::max(0.95 + 0.005 * k, 0.0195 * k));
-        const double slope = sh.nt == 1 ? (wide ? 0.0105 : 0.0061) : (wide ? 0.0195 : 0.0148);
+        const double slope = sh.nt == 1 ? (wide ? 0.0062 : 0.0051) : (wide ? 0.0195 : 0.0148);
         const double pieces4 = (wide ? 6.2 : 5.7) + (sh.nt - 1) * (wide ? 3.5 : 2.2) + 0.003 * k + std::max(items - 512, 0.0) * slope;
         return rows4 < pieces4 - (plans ? 0 : 2.5);  // (a planned call's draft rows: a launch of their own)
     }

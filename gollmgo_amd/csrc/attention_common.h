@@ -165,11 +165,21 @@ inline AttnShape attn_shape(const KV* kv, int rows, int num_q_heads) {
     return {true, (tiles + groups - 1) / groups, groups};
 }
 
-// The two for a pool. 4-bit ones: two workgroups per CU; chunks of 64 tokens, of 32 from three row
-// tiles on, which halve the chunk's scores, probabilities and scales next to the O tiles.
-__host__ __device__ constexpr int int4_chunk_tokens(int nt) { return nt <= 2 ? 64 : 32; }
-inline int attn_kv_chunk_tokens(const KV* kv, int nt) {
-    return kv->dtype == GG_DTYPE_INT4 ? int4_chunk_tokens(nt) : attn_chunk_tokens((int)dtype_bytes(kv->dtype), nt);
+// 4-bit pools: tokens of a chunk for nt row tiles and `items` workgroups' worth of work.
+//   - 64 at one or two row tiles, 32 from three on, which halve the chunk's scores, probabilities and
+//     scales next to the O tiles;
+//   - 32 at one row tile where the items outnumber two workgroups per CU: the kernel then fits four to
+//     a CU, and the start and merge of one item (6 µs of its 10 to 20) overlap the others'. Per planned
+//     call, 64 / 32 tokens: 512 sequences of 512 keys 81 / 63 µs, 256 of 1100 70 / 63, 128 of 2048 58 /
+//     56, 128 of 256-2048 38 / 33; with fewer items, which longer loads serve better: 64 of 4096
+//     54 / 58, one of 100000 40 / 55.
+inline int int4_chunk_tokens(int nt, long long items) {
+    return nt >= 3 || (nt == 1 && items > 2LL * device_cu_count()) ? 32 : 64;
+}
+// Tokens per chunk, and workgroups per CU that the schedule counts on, for a call on a pool.
+inline int attn_kv_chunk_tokens(const KV* kv, const AttnShape& sh, int num_seqs) {
+    if (kv->dtype == GG_DTYPE_INT4) return int4_chunk_tokens(sh.nt, (long long)num_seqs * kv->num_kv_heads * sh.groups);
+    return attn_chunk_tokens((int)dtype_bytes(kv->dtype), sh.nt);
 }
 inline int attn_kv_occupancy(const KV* kv, int nt) {
     return kv->dtype == GG_DTYPE_INT4 ? 2 : attn_occupancy((int)dtype_bytes(kv->dtype), nt, kv->head_dim);
@@ -232,7 +242,7 @@ AttnPlan attn_plan(const KV* kv, int num_seqs, int rows, int num_q_heads, int ma
 
 gg_status_t launch_attn_mfma(const AttnArgs& a, const KVView& kv, hipStream_t s);
 gg_status_t launch_attn_full(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s);
-gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s);
+gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, int tok, hipStream_t s);
 gg_status_t launch_append_from_tables(const AttnArgs& a, const KVView& kv, hipStream_t s);
 
 #ifdef __HIPCC__

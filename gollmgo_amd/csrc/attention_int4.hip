@@ -62,9 +62,9 @@ __device__ __forceinline__ uint4 less_zero(uint4 v, uint32_t z0, uint32_t z1, ui
 
 __device__ __forceinline__ uint32_t f16_pair(float a, float b) { return cvt_pk_f16(a, b); }
 
-template <int NT, int HD, bool PREC>
+template <int NT, int HD, bool PREC, int TOK>
 struct Int4Shared {
-    static constexpr int kTok = int4_chunk_tokens(NT);
+    static constexpr int kTok = TOK;
     static constexpr int kMM = HD / 32, kParts = PREC ? 2 : 1;
     uint4 q[kParts][NT][kMM][64];   // B operands of S
     uint32_t qz[NT * 16];           // -sum q of a row, two f16 parts
@@ -115,7 +115,7 @@ __device__ __forceinline__ void int4_piece_by_rows(const AttnArgs& a, const KVVi
 // The piece's queries: HD / 8 threads a row, eight dims (one K dword) each. Loaded before the piece's
 // keys and values (loads retire in order, so the staging then waits for these alone), and put into
 // LDS as MFMA operands, scaled row by row.
-template <int NT, int HD, bool PREC>
+template <int NT, int HD, bool PREC, int TOK>
 struct Int4Queries {
     static constexpr int kPer = HD / 8, kStep = 256 / kPer, kIt = (16 * NT + kStep - 1) / kStep;
     uint4 w[kIt][PREC ? 2 : 1];
@@ -138,7 +138,7 @@ struct Int4Queries {
         }
     }
 
-    __device__ __forceinline__ void stage(const AttnArgs& a, int rows, Int4Shared<NT, HD, PREC>& s) const {
+    __device__ __forceinline__ void stage(const AttnArgs& a, int rows, Int4Shared<NT, HD, PREC, TOK>& s) const {
         constexpr int kMM = HD / 32;
         const int ch = threadIdx.x % kPer;
 #pragma unroll
@@ -197,9 +197,9 @@ struct Int4Queries {
     }
 };
 
-template <int NT, int HD, bool PREC>
+template <int NT, int HD, bool PREC, int TOK>
 __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, const PieceDesc& d) {
-    constexpr int kTok = int4_chunk_tokens(NT), kNS = kTok / 16, kN = 4 * kNS;  // a chunk's tokens, S tiles; a lane's tokens
+    constexpr int kTok = TOK, kNS = kTok / 16, kN = 4 * kNS;  // a chunk's tokens, S tiles; a lane's tokens
     using IO = PieceIO<GG_DTYPE_INT8, kTok, HD>;    // (block ids of chunks)
     using Geom = Geo<1, kTok, HD>;                  // (tokens of lanes and S tiles)
     constexpr int kMM = HD / 32, kVT = HD / 32;     // K operands of a token; V loads of a lane
@@ -214,7 +214,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
     if (rows <= 0) return;
     const int first_masked = ctx - nrows;
     const int nchunks = (d.t_end - d.t0 + kTok - 1) / kTok;
-    __shared__ Int4Shared<NT, HD, PREC> s;
+    __shared__ Int4Shared<NT, HD, PREC, TOK> s;
 
     // The call's own rows in this piece: written first, by the whole workgroup. (Row groups write
     // the same bytes.)
@@ -265,7 +265,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             }
         }
     };
-    Int4Queries<NT, HD, PREC> qs;
+    Int4Queries<NT, HD, PREC, TOK> qs;
     const auto fb = IO::first_blocks(a, d);
     qs.load(a, kv, d, rows);
     LaneBlocks bl_cur = IO::lane_blocks(kv, fb.r0, d.t_end), bl_next = IO::lane_blocks(kv, fb.r1, d.t_end);
@@ -550,8 +550,8 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 // PLANNED: workgroup p runs the plan's piece p, and the last piece of a split item merges it. Else
 // workgroup (sequence, head) runs the whole item: calls too narrow to cut, and batches that the
 // plan does not rank.
-template <int NT, int HD, bool PREC, bool PLANNED>
-__global__ void __launch_bounds__(256, 2) attn_int4_kernel(AttnArgs a, KVView kv) {
+template <int NT, int HD, bool PREC, int TOK, bool PLANNED>
+__global__ void __launch_bounds__(256, NT == 1 && TOK == 32 ? 4 : 2) attn_int4_kernel(AttnArgs a, KVView kv) {
     const int heads = kv.Hkv * a.row_groups;
     if constexpr (PLANNED) {
         const int p = blockIdx.x;
@@ -559,42 +559,44 @@ __global__ void __launch_bounds__(256, 2) attn_int4_kernel(AttnArgs a, KVView kv
         if (e.x < 0) return;  // past the last piece
         const int h = e.y & 0xffff, np = e.y >> 16, row0 = h / kv.Hkv * (16 * NT);
         const PieceDesc d{e.x, h % kv.Hkv, e.z, e.w, -1, np > 1 ? f.z + f.w * heads : -1, row0, f.x, f.y};
-        int4_piece<NT, HD, PREC>(a, kv, d);
+        int4_piece<NT, HD, PREC, TOK>(a, kv, d);
         if (np > 1 && a.num_q_heads / kv.Hkv * d.nrows > row0) lpt_merge_if_last<HD>(a, kv.Hkv, heads, d, h, np, f.z, 16 * NT);
     } else {
         const int h = blockIdx.x % heads, b = blockIdx.x / heads;
         const int ctx = seq_keys(a, b, kBS), nrows = seq_rows(a, b);
-        int4_piece<NT, HD, PREC>(a, kv, PieceDesc{b, h % kv.Hkv, 0, ctx, -1, -1, h / kv.Hkv * (16 * NT), ctx, nrows});
+        int4_piece<NT, HD, PREC, TOK>(a, kv, PieceDesc{b, h % kv.Hkv, 0, ctx, -1, -1, h / kv.Hkv * (16 * NT), ctx, nrows});
     }
 }
 
-template <int NT, int HD, bool PREC>
+template <int NT, int HD, bool PREC, int TOK>
 void launch_one(const AttnArgs& a, const KVView& kv, hipStream_t s) {
     if (a.sched == ATTN_SCHED_LPT)
-        attn_int4_kernel<NT, HD, PREC, true><<<lpt_pieces(a.sk_grid, a.num_seqs, kv.Hkv * a.row_groups), 256, 0, s>>>(a, kv);
+        attn_int4_kernel<NT, HD, PREC, TOK, true><<<lpt_pieces(a.sk_grid, a.num_seqs, kv.Hkv * a.row_groups), 256, 0, s>>>(a, kv);
     else
-        attn_int4_kernel<NT, HD, PREC, false><<<a.num_seqs * kv.Hkv * a.row_groups, 256, 0, s>>>(a, kv);
+        attn_int4_kernel<NT, HD, PREC, TOK, false><<<a.num_seqs * kv.Hkv * a.row_groups, 256, 0, s>>>(a, kv);
 }
 
-template <int NT, int HD>
+template <int NT, int HD, int TOK>
 void launch_prec(const AttnArgs& a, const KVView& kv, hipStream_t s) {
-    if (a.q_dtype == GG_DTYPE_F32 || a.out_dtype == GG_DTYPE_F32) launch_one<NT, HD, true>(a, kv, s);
-    else launch_one<NT, HD, false>(a, kv, s);
+    if (a.q_dtype == GG_DTYPE_F32 || a.out_dtype == GG_DTYPE_F32) launch_one<NT, HD, true, TOK>(a, kv, s);
+    else launch_one<NT, HD, false, TOK>(a, kv, s);
+}
+
+// (int4_chunk_tokens: 64 or 32 at one row tile, 64 at two, 32 at three and four.)
+template <int HD>
+void launch_tiles(const AttnArgs& a, const KVView& kv, int nt, int tok, hipStream_t s) {
+    if (nt == 1 && tok == 64) launch_prec<1, HD, 64>(a, kv, s);
+    else if (nt == 1) launch_prec<1, HD, 32>(a, kv, s);
+    else if (nt == 2) launch_prec<2, HD, 64>(a, kv, s);
+    else if (nt == 3) launch_prec<3, HD, 32>(a, kv, s);
+    else if constexpr (HD == 64) launch_prec<4, HD, 32>(a, kv, s);
 }
 
 }  // namespace
 
-gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, hipStream_t s) {
-    if (kv.D == 128) {
-        if (sh.nt == 1) launch_prec<1, 128>(a, kv, s);
-        else if (sh.nt == 2) launch_prec<2, 128>(a, kv, s);
-        else launch_prec<3, 128>(a, kv, s);
-    } else {
-        if (sh.nt == 1) launch_prec<1, 64>(a, kv, s);
-        else if (sh.nt == 2) launch_prec<2, 64>(a, kv, s);
-        else if (sh.nt == 3) launch_prec<3, 64>(a, kv, s);
-        else launch_prec<4, 64>(a, kv, s);
-    }
+gg_status_t launch_attn_int4(const AttnArgs& a, const KVView& kv, const AttnShape& sh, int tok, hipStream_t s) {
+    if (kv.D == 128) launch_tiles<128>(a, kv, sh.nt, tok, s);
+    else launch_tiles<64>(a, kv, sh.nt, tok, s);
     return check_hip(hipGetLastError(), "verify_attention launch");
 }
 

@@ -384,12 +384,12 @@ gg_status_t launch_attn_mfma(const AttnArgs& a, const KVView& kv, hipStream_t s)
     const AttnShape sh = attn_shape(a.kv, a.rows, a.num_q_heads);
     const int G = a.num_q_heads / kv.Hkv;
     const int nt = sh.nt;
-    const int tok = attn_kv_chunk_tokens(a.kv, nt);
+    const int tok = attn_kv_chunk_tokens(a.kv, sh, a.num_seqs);
     if (a.sched == ATTN_SCHED_LPT && !a.plan_ready) {
         const gg_status_t st = launch_attn_plan(a, s);
         if (st != GG_OK) return st;
     }
-    if (kv.dt == GG_DTYPE_INT4) return launch_attn_int4(a, kv, sh, s);
+    if (kv.dt == GG_DTYPE_INT4) return launch_attn_int4(a, kv, sh, tok, s);
     if (sh.full) return launch_attn_full(a, kv, sh, s);
     gg_status_t st;
     switch (kv.dt) {
@@ -413,7 +413,7 @@ gg_status_t launch_attn_plan(const AttnArgs& a, hipStream_t s) {
     const int Hkv = kv->num_kv_heads;
     const AttnShape sh = attn_shape(kv, a.rows, a.num_q_heads);
     const int heads = Hkv * sh.groups;
-    const int tok = attn_kv_chunk_tokens(kv, sh.nt);
+    const int tok = attn_kv_chunk_tokens(kv, sh, a.num_seqs);
     const int pieces = lpt_pieces(a.sk_grid, a.num_seqs, heads);
     const int tok_log2 = tok == 64 ? 6 : 5, tmin = lpt_min_chunks_of(kv, tok);
     if (a.num_seqs <= 256) attn_lpt_plan_kernel<256><<<1, 256, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces);
