@@ -324,6 +324,25 @@ static gg_status_t rope_args(RopeArgs& a, const char* who, const void* q, long l
     return GG_OK;
 }
 
+// Outputs that overlap an input are read after they are written, but for rows turned in place: each wave
+// reads its own whole.
+static gg_status_t rope_overlaps(const RopeArgs& a, const char* who) {
+    const long long eb = (long long)dtype_bytes(a.dt);
+    struct Span { uintptr_t lo, hi; };
+    auto span = [&](const void* p, int heads, long long stride) {
+        const uintptr_t lo = (uintptr_t)p;
+        return Span{lo, heads && p ? lo + (uintptr_t)(((a.n - 1) * stride + (long long)heads * a.D) * eb) : lo};
+    };
+    auto meet = [](const Span& x, const Span& y) { return x.lo < y.hi && y.lo < x.hi; };
+    const long long qw = (long long)a.Hq * a.D, kw = (long long)a.Hkv * a.D;
+    const Span q = span(a.q, a.Hq, a.q_stride), k = span(a.k, a.Hkv, a.k_stride), v = span(a.v, a.Hkv, a.v_stride),
+               qo = span(a.q_out, a.Hq, qw), ko = span(a.k_out, a.Hkv, kw);
+    const bool q_in_place = a.q_out == a.q && (a.q_stride == qw || a.n == 1), k_in_place = a.k_out == a.k && (a.k_stride == kw || a.n == 1);
+    if ((meet(qo, q) && !q_in_place) || (meet(ko, k) && !k_in_place) || meet(qo, k) || meet(qo, v) || meet(ko, q) || meet(qo, ko))
+        return fail(GG_ERR_INVALID, std::string(who) + ": an output overlaps an input or the other output");
+    return GG_OK;
+}
+
 GG_API gg_status_t gg_qk_norm_rope(const void* q, long long q_stride, const void* k, long long k_stride,
                                    gg_dtype_t dtype, int n_rows, int num_q_heads, int num_kv_heads, int head_dim,
                                    const void* q_weight, const void* k_weight, float eps, const int32_t* positions,
@@ -338,6 +357,8 @@ GG_API gg_status_t gg_qk_norm_rope(const void* q, long long q_stride, const void
     if (n_rows == 0) return GG_OK;
     GG_CHECK_ARG(num_kv_heads == 0 || k_out, "gg_qk_norm_rope: NULL buffer");
     a.k_out = k_out;
+    const gg_status_t apart = rope_overlaps(a, "gg_qk_norm_rope");
+    if (apart != GG_OK) return apart;
     return launch_qk_norm_rope(a, nullptr, 0, (hipStream_t)stream);
 }
 
@@ -361,11 +382,13 @@ GG_API gg_status_t gg_qk_norm_rope_append(gg_kv_t kv, int layer, const void* q, 
                  "gg_qk_norm_rope_append: rows overlap (stride below heads * head_dim)");
     if (n_rows == 0) return GG_OK;
     GG_CHECK_ARG(v && slot_mapping, "gg_qk_norm_rope_append: NULL buffer");
-    const gg_status_t dev = on_pool_device(kv, "gg_qk_norm_rope_append");
-    if (dev != GG_OK) return dev;
     a.v = v;
     a.v_stride = v_stride;
     a.slots = slot_mapping;
+    const gg_status_t apart = rope_overlaps(a, "gg_qk_norm_rope_append");
+    if (apart != GG_OK) return apart;
+    const gg_status_t dev = on_pool_device(kv, "gg_qk_norm_rope_append");
+    if (dev != GG_OK) return dev;
     return launch_qk_norm_rope(a, kv, layer, (hipStream_t)stream);
 }
 

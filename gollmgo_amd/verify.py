@@ -67,6 +67,15 @@ def _rows(t: torch.Tensor, name: str):
     return t.data_ptr(), sn if n > 1 else h * d
 
 
+def _here(*tensors):
+    """Refuses tensors of another device than the current one, where the call runs (None and host
+    tensors are left to the other checks)."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.get_device() != here:
+            raise ValueError("a tensor is on another device than the current one")
+
+
 _STYLES = {"halves": int(RopeStyle.HALVES), "pairs": int(RopeStyle.PAIRS)}
 
 
@@ -79,8 +88,6 @@ def _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style):
         raise ValueError("q or k is needed")
     if some.dim() != 3 or (k is not None and k.dim() != 3):
         raise ValueError("q and k must be [n_rows, heads, head_dim]")
-    if some.is_cuda and some.get_device() != torch.cuda.current_device():
-        raise ValueError("the rows are on another device than the current one")
     n, _, d = some.shape
     dtype = some.dtype
     if k is not None and k is not some:
@@ -102,7 +109,8 @@ def _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style):
             raise ValueError("k_weight must be [head_dim] of the rows' dtype")
         wk = _dev(k_weight, "k_weight")
     if pair_axis is not None:
-        axis = bytes(pair_axis)  # (ValueError for what is no small whole number)
+        # (ValueError or TypeError for what are no small whole numbers)
+        axis = pair_axis if type(pair_axis) is bytes else bytes(list(pair_axis))
         if len(axis) != pairs or (pairs and max(axis) >= axes):
             raise ValueError("pair_axis must name an axis of positions for each of inv_freq's pairs")
     elif axes != 1:
@@ -135,6 +143,7 @@ def qk_norm_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], positions
     "halves": dim j with j + pairs; "pairs": 2j with 2j + 1. -> (q_out, k_out), contiguous;
     q_out may be q itself where that is contiguous."""
     dt, n, d, wq, wk, rest = _turn(q, k, positions, inv_freq, q_weight, k_weight, pair_axis, style)
+    _here(q, k, positions, inv_freq, q_weight, k_weight, q_out, k_out)
     qp = kp = qo = ko = None
     qs = ks = hq = hk = 0
     if q is not None:
@@ -267,6 +276,7 @@ class KVCache:
             raise ValueError("k and v must be [n_rows, num_kv_heads, head_dim] of one dtype")
         if slot_mapping.numel() != n:
             raise ValueError("slot_mapping must be [n_rows]")
+        _here(q, k, v, positions, inv_freq, slot_mapping, q_weight, k_weight, q_out)
         kp, ks = _rows(k, "k")
         vp, vs = _rows(v, "v")
         qp = qo = None
@@ -293,6 +303,7 @@ class KVCache:
             v = torch.empty_like(k)
         else:
             k, v = out
+        _here(slot_mapping, k, v)
         kind, ptrs = None, []
         for t, name in ((k, "k"), (v, "v")):
             if t is None:

@@ -159,7 +159,8 @@ gg_status_t gg_kv_set_head_scales(gg_kv_t kv, int layer, const float* k_scales,
  * paged_kv_write_{f16,bf16} kernels (kernels/gollmgo_paged_attn.cu:14-35,126-146).
  *   k, v         : device [n_rows][num_kv_heads][head_dim] of src_dtype (F32/F16/BF16)
  *   slot_mapping : device int32[n_rows]; slot = block*block_size + offset; a
- *                  negative slot skips the row.
+ *                  negative slot skips the row. Two rows of one call must not share a
+ *                  slot (what such a slot holds then belongs to neither).
  * PER_BLOCK pools: rows that land in the same block in one call must be adjacent
  * in slot_mapping (skipped rows may sit between them) with increasing offsets (as
  * BlockTable.Append produces them,
@@ -186,13 +187,15 @@ gg_status_t gg_kv_append(gg_kv_t kv, int layer, const void* k, const void* v,
  *                 t * {q,k}_stride + h * head_dim, so slices of a fused projection are
  *                 taken as they are (strides in elements, at least heads * head_dim)
  *   q_out, k_out: device [n_rows][heads][head_dim] of dtype, contiguous. q_out may be q
- *                 (and k_out k) where that is contiguous; other overlaps are not allowed.
+ *                 (and k_out k) where that is contiguous; other overlaps of an output with
+ *                 an input or the other output are refused.
  *   positions   : device int32[num_axes][n_rows], num_axes 1..8
  *   pair_axis   : HOST uint8[num_pairs], the axis of each pair (copied by the call), or
  *                 NULL for axis 0
  *   inv_freq    : device float[num_pairs], 2 * num_pairs <= head_dim <= 1024, num_pairs
  *                 0..512
  *   q_weight, k_weight: device [head_dim] of dtype, or NULL; eps >= 0, finite
+ * n_rows 0 (nothing to do) to 2^24; a call past one launch's 2^32 threads: GG_ERR_INVALID.
  * num_q_heads or num_kv_heads may be 0 (the other side alone; its pointers are not used). */
 typedef enum {
     GG_ROPE_HALVES = 0,
@@ -226,7 +229,8 @@ gg_status_t gg_qk_norm_rope_append(gg_kv_t kv, int layer, const void* q, long lo
  * [n_rows][num_kv_heads][head_dim] of out_dtype F32/F16/BF16; either may be NULL) is what
  * the pool holds in slot_mapping[i], its scales applied in fp32 and rounded once. For
  * kernels that take dense K/V, and to look at a cache. A row whose slot is negative or
- * past the pool is left as it was. The inverse of gg_kv_append in its arguments; no
+ * past the pool is left as it was. n_rows 0 to 2^24, and no more than one launch holds (2^32
+ * threads) or GG_ERR_INVALID. The inverse of gg_kv_append in its arguments; no
  * counterpart in the reference (whose pools hold the source type). */
 gg_status_t gg_kv_read(gg_kv_t kv, int layer, void* k_out, void* v_out, gg_dtype_t out_dtype,
                        const int32_t* slot_mapping, int n_rows, void* stream);

@@ -250,6 +250,39 @@ def test_refusals(gv):
     kv.close()
 
 
+def test_tensors_of_another_device_are_refused(gv, monkeypatch):
+    """The current device, as the calls see it, is one that holds none of the tensors."""
+    n, hq, h, d = 4, 4, 2, 64
+    q, k = torch.zeros(n, hq, d, device="cuda"), torch.zeros(n, h, d, device="cuda")
+    pos, freq = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.ones(32, device="cuda")
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    kv = gv.KVCache(1, 2, 16, h, d, DType.INT4)
+    out = (torch.zeros(n, h, d, device="cuda"), None)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "current_device", lambda: 1)
+        for call in (lambda: gv.qk_norm_rope(q, k, pos, freq), lambda: kv.norm_rope_append(0, q, k, k, pos, freq, slots),
+                     lambda: kv.read(0, slots, out=out)):
+            with pytest.raises(ValueError, match="another device"):
+                call()
+    kv.close()
+
+
+def test_axes_of_pairs_in_any_form(gv):
+    """Bytes, lists, arrays and tensors of whole numbers name the same axes; anything else is refused."""
+    rng = np.random.default_rng(11)
+    n, d = 5, 64
+    q = torch.from_numpy(rng.normal(0, 1, (n, 2, d)).astype(np.float32)).cuda()
+    pos = torch.from_numpy(rng.integers(0, 1000, (2, n)).astype(np.int32)).cuda()
+    freq = torch.from_numpy(np.exp2(-rng.uniform(0, 10, 32)).astype(np.float32)).cuda()
+    axes = [int(x) for x in rng.integers(0, 2, 32)]
+    want = gv.qk_norm_rope(q, None, pos, freq, pair_axis=axes)[0]
+    for form in (bytes(axes), tuple(axes), np.array(axes), np.array(axes, dtype=np.uint8), torch.tensor(axes)):
+        assert torch.equal(gv.qk_norm_rope(q, None, pos, freq, pair_axis=form)[0], want)
+    for bad in (32, np.array(axes) / 2, [300] * 32):
+        with pytest.raises((ValueError, TypeError)):
+            gv.qk_norm_rope(q, None, pos, freq, pair_axis=bad)
+
+
 def test_graph_of_a_layer(gv):
     """Norm, rotation and append into the pool, plan and attention: captured once, replayed."""
     rng = np.random.default_rng(6)

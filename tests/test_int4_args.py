@@ -68,3 +68,19 @@ def test_norm_rope_append_refuses_no_handle():
     assert lib.gg_qk_norm_rope_append(None, 0, 1, 256, 1, 128, 1, 128, 0, 4, 4, None, None, 1e-6, 1, 1, None, 1, 32, 0, 1, 1,
                                       None) == Status.ERR_INVALID
     assert "kv is NULL" in _lib.last_error()
+
+
+# (4 rows of 4 query heads, 2 kv heads of 64 fp32 values: 1024 bytes a query row, 512 a key row.)
+Q, K, QO, KO = 0x10000, 0x20000, 0x30000, 0x40000
+
+
+@pytest.mark.parametrize("bad", [
+    dict(qo=Q + 4), dict(qo=Q + 4095), dict(qo=Q - 4095), dict(qo=Q, qs=512), dict(ko=K, ks=256), dict(ko=K + 2047),
+    dict(qo=K + 2047), dict(qo=K - 4095), dict(ko=Q), dict(ko=Q + 4092), dict(ko=QO + 4095), dict(qo=KO),
+    dict(k=Q + 1024, qs=384, ks=384, qo=Q + 1536),
+])
+def test_norm_rope_refuses_overlaps(bad):
+    a = dict(q=Q, k=K, qo=QO, ko=KO)
+    a.update(bad)
+    assert rope_call(**a) == Status.ERR_INVALID
+    assert "overlaps" in _lib.last_error()
