@@ -17,12 +17,32 @@ constexpr int kRowsMaxD = 1024;
 constexpr int kRopeWaves = 4096;  // waves that fill the machine (heads_per_wave)
 
 // cos and sin of position times frequency. The angle in turns, and its whole turns taken off, in 64
-// bits (at position 2^31 the product still keeps 2^-21 of a turn); the rest is exact enough in fp32.
+// bits (at position 2^31 the product still keeps 2^-21 of a turn). The rest goes to fp32 as a value and
+// what its rounding left, which turns the result once more by less than 2^-23.
 __device__ __forceinline__ void turn_of(int pos, float freq, float& c, float& s) {
     constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
     double t = (double)pos * ((double)freq * kTurn);
     t -= __builtin_rint(t);
-    sincospif((float)(2.0 * t), &s, &c);
+    t += t;
+    const float half_turns = (float)t, rest = (float)(t - (double)half_turns) * 3.14159265f;
+    float s0, c0;
+    sincospif(half_turns, &s0, &c0);
+    c = __builtin_fmaf(-s0, rest, c0);
+    s = __builtin_fmaf(c0, rest, s0);
+}
+
+// A normed element, and a pair turned: every kernel here rounds the same products in the same order.
+// (Rounded one by one, not fused: a key whose quotient by its pool's step falls on a tie then goes the
+// way that the same formula in plain fp32 takes it, where its norm has the same last bit.)
+__device__ __forceinline__ float normed(float x, float r, float w) {
+#pragma clang fp contract(off)
+    return x * r * w;
+}
+__device__ __forceinline__ void turn_pair(float& p, float& q, float c, float s) {
+#pragma clang fp contract(off)
+    const float x = p * c - q * s, y = q * c + p * s;
+    p = x;
+    q = y;
 }
 
 __device__ __forceinline__ int pair_axis(const RopeArgs& a, int j) { return (a.axis[j >> 3] >> (4 * (j & 7))) & 15; }
@@ -82,7 +102,7 @@ __device__ __forceinline__ void rows_wave(const RopeArgs& a, const PoolOut& p, i
     const float kinv = cached && p.dt == GG_DTYPE_FP8_E4M3 ? p.k_inv[h] : 1.f;
     auto value = [&](int d) {
         const float x = load_as_f32(src, a.dt, at + d);
-        return weight ? x * norm * load_as_f32(weight, a.dt, d) : x;
+        return weight ? normed(x, norm, load_as_f32(weight, a.dt, d)) : x;
     };
     auto put = [&](int d, float y) {
         if (to_int4) s_row[d] = y;
@@ -97,9 +117,10 @@ __device__ __forceinline__ void rows_wave(const RopeArgs& a, const PoolOut& p, i
         const int da = a.style == GG_ROPE_PAIRS ? 2 * u : u, db = a.style == GG_ROPE_PAIRS ? 2 * u + 1 : u + P;
         float c, s;
         turn_of(a.positions[(size_t)pair_axis(a, u) * a.n + t], a.inv_freq[u], c, s);
-        const float x = value(da), y = value(db);
-        put(da, x * c - y * s);
-        put(db, y * c + x * s);
+        float x = value(da), y = value(db);
+        turn_pair(x, y, c, s);
+        put(da, x);
+        put(db, y);
     }
     if (!cached) return;
     const size_t vat = (size_t)t * a.v_stride + (size_t)h * D;
@@ -174,36 +195,25 @@ __device__ __forceinline__ void apply_turn(const RopeArgs& a, const Unit& x, con
     if (!x.turned) return;
     if (a.style == GG_ROPE_HALVES) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float p = fa[e], q = fb[e];
-            fa[e] = p * r.c[e] - q * r.s[e];
-            fb[e] = q * r.c[e] + p * r.s[e];
-        }
+        for (int e = 0; e < 4; ++e) turn_pair(fa[e], fb[e], r.c[e], r.s[e]);
     } else {
-        auto two = [](float& p, float& q, float c, float s) {
-            const float x = p, y = q;
-            p = x * c - y * s;
-            q = y * c + x * s;
-        };
-        two(fa[0], fa[1], r.c[0], r.s[0]);
-        two(fa[2], fa[3], r.c[1], r.s[1]);
-        two(fb[0], fb[1], r.c[2], r.s[2]);
-        two(fb[2], fb[3], r.c[3], r.s[3]);
+        turn_pair(fa[0], fa[1], r.c[0], r.s[0]);
+        turn_pair(fa[2], fa[3], r.c[1], r.s[1]);
+        turn_pair(fb[0], fb[1], r.c[2], r.s[2]);
+        turn_pair(fb[2], fb[3], r.c[3], r.s[3]);
     }
 }
-// A row's two runs, normed (w: the weight's runs; none where has is false).
+// A row's two runs, normed (w: the weight's runs), by the row's LPR lanes together.
 template <int LPR>
-__device__ __forceinline__ void norm_runs(const RopeArgs& a, bool has, const float (&wa)[4], const float (&wb)[4], float (&fa)[4],
-                                          float (&fb)[4]) {
+__device__ __forceinline__ void norm_runs(const RopeArgs& a, const float (&wa)[4], const float (&wb)[4], float (&fa)[4], float (&fb)[4]) {
     float sum = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
     const float r = rsqrtf(__builtin_fmaf(group_sum<LPR>(sum), a.inv_d, a.eps));
-    if (!has) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        fa[e] = fa[e] * r * wa[e];
-        fb[e] = fb[e] * r * wb[e];
+        fa[e] = normed(fa[e], r, wa[e]);
+        fb[e] = normed(fb[e], r, wb[e]);
     }
 }
 template <gg_dtype_t T>
@@ -213,8 +223,7 @@ __device__ __forceinline__ void weight_runs(const void* w, const Unit& x, float 
 }
 
 // Heads [h0, h1) of one side (queries or keys) of row t by one wave, 64 / LPR at a time, four steps in
-// flight. A turned element is r (x w cos +- x' w' sin), x' the pair's other end and r the head's norm:
-// the products of weights and cosines are formed once for all heads.
+// flight.
 template <gg_dtype_t T, int LPR>
 __device__ __forceinline__ void dense_side(const RopeArgs& a, const Unit& x, const Turn& r, const void* rows, long long stride,
                                            const void* weight, void* out, int heads, int t, int h0, int h1) {
@@ -238,18 +247,6 @@ __device__ __forceinline__ void dense_side(const RopeArgs& a, const Unit& x, con
     for (int i = 0; i < kAhead; ++i) fetch(i, i * kRPW);
     float wa[4] = {1.f, 1.f, 1.f, 1.f}, wb[4] = {1.f, 1.f, 1.f, 1.f};
     if (weight && x.live) weight_runs<T>(weight, x, wa, wb);
-    // Pair e of the lane's four: its ends' weights.
-    float c0[4], c1[4], s0[4], s1[4];  // (first end: x c0 - x' s0; second: x' c1 + x s1)
-    const bool halves = a.style == GG_ROPE_HALVES;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float w0 = halves ? wa[e] : e < 2 ? wa[2 * e] : wb[2 * (e & 1)];
-        const float w1 = halves ? wb[e] : e < 2 ? wa[2 * e + 1] : wb[2 * (e & 1) + 1];
-        c0[e] = w0 * r.c[e];
-        s1[e] = w0 * r.s[e];
-        c1[e] = w1 * r.c[e];
-        s0[e] = w1 * r.s[e];
-    }
     for (int hb = 0; hb < h1 - h0; hb += kAhead * kRPW) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
@@ -259,31 +256,8 @@ __device__ __forceinline__ void dense_side(const RopeArgs& a, const Unit& x, con
             to_f32<T>(ra[i], fa);
             to_f32<T>(rb[i], fb);
             fetch(i, h + kAhead * kRPW);
-            float k = 1.f;
-            if (weight) {
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
-                k = rsqrtf(__builtin_fmaf(group_sum<LPR>(sum), a.inv_d, a.eps));
-            }
-            if (!x.turned) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    fa[e] = fa[e] * wa[e] * k;
-                    fb[e] = fb[e] * wb[e] * k;
-                }
-            } else {
-                auto pair = [&](float& p, float& q, int e) {
-                    const float u = (p * c0[e] - q * s0[e]) * k, v = (q * c1[e] + p * s1[e]) * k;
-                    p = u;
-                    q = v;
-                };
-                if (halves) {
-                    pair(fa[0], fb[0], 0), pair(fa[1], fb[1], 1), pair(fa[2], fb[2], 2), pair(fa[3], fb[3], 3);
-                } else {
-                    pair(fa[0], fa[1], 0), pair(fa[2], fa[3], 1), pair(fb[0], fb[1], 2), pair(fb[2], fb[3], 3);
-                }
-            }
+            if (weight) norm_runs<LPR>(a, wa, wb, fa, fb);
+            apply_turn(a, x, r, fa, fb);
             if (h < n) {
                 store4<T>(dst, x.oa, fa);
                 store4<T>(dst, x.ob, fb);
@@ -341,7 +315,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4
             to_f32<T>(w.kb, kb);
             to_f32<T>(w.va, va);
             to_f32<T>(w.vb, vb);
-            norm_runs<LPR>(a, a.k_weight != nullptr, wa, wb, ka, kb);
+            if (a.k_weight) norm_runs<LPR>(a, wa, wb, ka, kb);
             apply_turn(a, x, r, ka, kb);
             oa = x.oa;
             ob = x.ob;
