@@ -165,14 +165,22 @@ __device__ __forceinline__ int lpt_place(int u, int rg, int units, int groups) {
     return first * groups + rg * min(8, units - first) + (u & 7);
 }
 
-// One workgroup of N threads (one sequence per thread): sizes, ranks and lays out the pieces.
-// A chain of barriers and short loops of one workgroup, paid once per step: N is 256 for up
-// to 256 sequences (four waves meet at its barriers), the table is written by all threads, and
+// Workgroups of N threads (one sequence per thread), each of which sizes all sequences and ranks and
+// lays out the pieces of its share of them. A chain of barriers and short loops, paid once per step: N
+// is 256 for up to 256 sequences (four waves meet at its barriers), the table is written by all threads, and
 // no 64-bit division is left (the fp64 quotients are exact where rounding matters: both
 // operands are integers below 2^53 and no non-integer quotient comes within 2^-28 of one).
-// Per call, 64 sequences 9.4 -> 7.6 µs, one 6.7 -> 5.2.
+// Several workgroups against one, 8 kv heads, kernel time: 128 sequences 12.4 -> 5.5 µs, 64 8.6 -> 4.9,
+// 32 6.7 -> 6.1, one (one workgroup still) 4.2 -> 4.4; shares of 64 items the same as of 128.
+constexpr int kPlanItems = 128, kPlanGroups = 16;  // items of a workgroup's share; most workgroups
+struct PlanShare {
+    int span;        // sequences of a workgroup
+    int lanes_log2;  // lanes to rank one
+    int sub_log2;    // threads to write one of its items
+};
 template <int N>
-__global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, int tok_log2, int tmin, int slots, int pieces) {
+__global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, int tok_log2, int tmin, int slots, int pieces,
+                                                            PlanShare share) {
     __shared__ __align__(16) int s_key[N];  // piece size in chunks (0: no work)
     __shared__ __align__(16) int s_cnt[N];  // pieces of the sequence over all kv heads
     __shared__ int s_nch[N], s_ctx[N], s_rows[N], s_first[N], s_pos[N], s_np[N];
@@ -228,42 +236,48 @@ __global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, i
     const unsigned long long before = block_excl_scan2<N>(nfull, np > 1 ? np * Hkv : 0, s_scan, &sums);
     const int full_pos = (int)(unsigned)before, F = (int)(unsigned)sums;  // (its barrier publishes s_key / s_cnt)
     s_first[b] = (int)(before >> 32);
-    // Pieces ahead of this sequence's: larger ones, then equal ones of lower sequences. Eight
-    // sequences per step from 16-byte LDS reads (independent adds, no serial chain).
-    int pos = F, all = F;
-    if (b < B || b == 0) {
-        for (int t0 = 0; t0 < B; t0 += 8) {
+    s_np[b] = np | (full_pos << 10);
+    // This workgroup's sequences, and the pieces ahead of each: larger ones, then equal ones of lower
+    // sequences. As many lanes to a sequence as there are threads for, eight others per step from
+    // 16-byte LDS reads (independent adds, no serial chain).
+    const int q0 = (int)blockIdx.x * share.span, q1 = min(B, q0 + share.span), g = 1 << share.lanes_log2;
+    const int mine = q0 + ((int)threadIdx.x >> share.lanes_log2);
+    if (mine < q1) {
+        const int my_key = s_key[mine];
+        int pos = 0, all = 0;
+        for (int t0 = 8 * ((int)threadIdx.x & (g - 1)); t0 < B; t0 += 8 * g) {
             const int4 k0 = *(const int4*)&s_key[t0], k1 = *(const int4*)&s_key[t0 + 4];
             const int4 n0 = *(const int4*)&s_cnt[t0], n1 = *(const int4*)&s_cnt[t0 + 4];
             const int kk[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
             const int nn[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int t = t0 + e;
-                pos += (kk[e] > key || (kk[e] == key && t < b)) ? nn[e] : 0;
+                pos += (kk[e] > my_key || (kk[e] == my_key && t0 + e < mine)) ? nn[e] : 0;
                 all += nn[e];
             }
         }
-        if (b == 0) s_t = all;
+        for (int o = 1; o < g; o <<= 1) {
+            pos += __shfl_xor(pos, o);
+            all += __shfl_xor(all, o);
+        }
+        if (((int)threadIdx.x & (g - 1)) == 0) s_pos[mine] = F + pos;
+        if (threadIdx.x == 0) s_t = F + all;
     }
-    s_pos[b] = pos;
-    s_np[b] = np | (full_pos << 10);
     __syncthreads();
     const int total = s_t;
-    // The table, by all threads: several per (sequence, kv head) when those are few.
+    // Its part of the table, by all threads: several per (sequence, kv head) when those are few.
     int* plan = a.plan;
     int4* table = (int4*)lpt_table(plan);
     const int heads = B * Hkv;
     const int kvh_n = Hkv / a.row_groups;
-    int sub = 1;
-    while (sub * 2 * heads <= N) sub *= 2;
-    for (int i = threadIdx.x; i < heads * sub; i += N) {
-        const int item = i / sub, q = item / Hkv, h = item % Hkv;
+    const int sub = 1 << share.sub_log2;
+    for (int i = threadIdx.x; i < (q1 - q0) * Hkv * sub; i += N) {
+        const int k = i >> share.sub_log2, q = q0 + k / Hkv, h = k % Hkv, item = q * Hkv + h;
         const int n = s_nch[q], qc = s_ctx[q], qr = s_rows[q], first = s_first[q] + h, qp = s_pos[q];
         const int qn = s_np[q] & 1023, qf = s_np[q] >> 10;
-        if (i % sub == 0) lpt_count(plan, pieces)[item] = 0;
+        if ((i & (sub - 1)) == 0) lpt_count(plan, pieces)[item] = 0;
         const int size = few && qn ? n / qn : T, extra = few ? n - size * qn : 0;
-        for (int j = i % sub; j < qn; j += sub) {
+        for (int j = i & (sub - 1); j < qn; j += sub) {
             const int c0 = j * size + min(j, extra);
             const int c1 = few ? c0 + size + (j < extra ? 1 : 0) : min(c0 + size, n);
             // Equal pieces of a sequence have a block of ranks: few, all of them; else its full
@@ -278,7 +292,7 @@ __global__ void __launch_bounds__(N) attn_lpt_plan_kernel(AttnArgs a, int Hkv, i
         }
     }
     // Entries past the last piece tell their workgroups to exit.
-    for (int q = total + threadIdx.x; q < pieces; q += N) table[2 * q] = make_int4(-1, 0, 0, 0);
+    for (int q = total + (int)(blockIdx.x * N + threadIdx.x); q < pieces; q += (int)gridDim.x * N) table[2 * q] = make_int4(-1, 0, 0, 0);
 }
 
 template <gg_dtype_t DT>
@@ -416,8 +430,15 @@ gg_status_t launch_attn_plan(const AttnArgs& a, hipStream_t s) {
     const int tok = attn_kv_chunk_tokens(kv, sh, a.num_seqs);
     const int pieces = lpt_pieces(a.sk_grid, a.num_seqs, heads);
     const int tok_log2 = tok == 64 ? 6 : 5, tmin = lpt_min_chunks_of(kv, tok);
-    if (a.num_seqs <= 256) attn_lpt_plan_kernel<256><<<1, 256, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces);
-    else attn_lpt_plan_kernel<kLptMaxSeqs><<<1, kLptMaxSeqs, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces);
+    // Shares of equal size, none of them empty.
+    const int threads = a.num_seqs <= 256 ? 256 : kLptMaxSeqs;
+    const int most = std::min((a.num_seqs * heads + kPlanItems - 1) / kPlanItems, std::min(a.num_seqs, kPlanGroups));
+    PlanShare share{(a.num_seqs + most - 1) / most, 0, 0};
+    const int groups = (a.num_seqs + share.span - 1) / share.span;
+    while (share.lanes_log2 < 5 && (share.span << (share.lanes_log2 + 1)) <= threads) ++share.lanes_log2;
+    while (((share.span * heads) << (share.sub_log2 + 1)) <= threads) ++share.sub_log2;
+    if (threads == 256) attn_lpt_plan_kernel<256><<<groups, 256, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces, share);
+    else attn_lpt_plan_kernel<kLptMaxSeqs><<<groups, kLptMaxSeqs, 0, s>>>(a, heads, tok_log2, tmin, a.sk_grid, pieces, share);
     return check_hip(hipGetLastError(), "verify_attention plan launch");
 }
 
