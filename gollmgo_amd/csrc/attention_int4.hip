@@ -2,8 +2,8 @@
 //
 // A 256-thread workgroup takes one piece of an item (a sequence, a kv head and up to 16 * NT of its
 // G * R query rows): the plan's pieces as in attention_mfma.h, or the whole item where nothing would
-// be cut. Its four waves stream disjoint chunks of 64 tokens (four blocks) and merge at the end.
-// Lane = 16 * g4 + c16.
+// be cut. Its four waves stream disjoint chunks of 64 or 32 tokens (int4_chunk_tokens) and merge at the
+// end. Lane = 16 * g4 + c16. Below, chunks of 64 (four blocks).
 //
 // Mathematics. A token's key is s_k (n - z_k) and its value s_v (m - z_v), n and m whole 0..15.
 //   score     = s_k (sum q n - z_k sum q): the products run over the codes alone. The zero point is
@@ -26,12 +26,21 @@
 //
 // p s_v is held in f16 in units of B 2^-10, B a power of two at or above every s_v the wave has seen
 // (O is rescaled when it grows). Values whose scales lie up to 2^12 apart keep 11 bits down to
-// p = 2^-12 that way, and half a step of 2^-35 B below; a piece whose scales lie further apart is computed row by row in fp32. Each
-// query row has a power of two of its own (its largest |q| in [2^7, 2^8)), so rows do not touch.
+// p = 2^-12 that way, and half a step of 2^-35 B below; a piece whose scales lie further apart is
+// computed row by row in fp32. Each query row has a power of two of its own (its largest |q| in
+// [2^7, 2^8)), so rows do not touch.
 // PREC (fp32 queries or outputs): queries and p s_v in two f16 parts each, 22 bits, and the zero points
 // are taken from the codes in the operands (f16, exact). Summed apart, codes and zero points leave a
 // rounding of 2^-20 of the row's range, which f16 probabilities hide and fp32 results would show;
 // subtracting is 64 + 16 * 4 instructions more a chunk.
+//
+// Bound: one read of a token's 2 * (D / 2) + 4 bytes serves all its kv head's rows. Planned calls, 8 kv
+// heads of 128, bf16, kernel time: 64 sequences of 1024-8192 keys, 24 rows a head (two row tiles),
+// 346 MB 72 µs, 4.8 TB/s (the same loads with nothing done to them 5.0 over the whole call); 128
+// sequences of 256-2048 keys, four rows 29.3 µs, 5.2 TB/s. Memory, both. 8 sequences of 16384-32768
+// keys, 36 rows (three row tiles) 77 µs, 2.8 TB/s: per SIMD 39 µs of vector and 19 of matrix
+// instructions, two waves to overlap them. One sequence of 3006 keys, 20 rows 17 µs: a chain of round
+// trips (table, block ids, keys and values, the pieces' records).
 #include "attention_mfma.h"
 #include "lanes.h"
 

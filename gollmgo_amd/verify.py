@@ -72,7 +72,7 @@ def _here(*tensors):
     tensors are left to the other checks)."""
     here = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.is_cuda and t.get_device() != here:
+        if t is not None and t.get_device() not in (here, -1):
             raise ValueError("a tensor is on another device than the current one")
 
 
