@@ -16,24 +16,43 @@ namespace {
 constexpr int kRowsMaxD = 1024;
 constexpr int kRopeWaves = 4096;  // waves that fill the machine (heads_per_wave)
 
-// cos and sin of position times frequency. The angle in turns, and its whole turns taken off, in 64
-// bits (at position 2^31 the product still keeps 2^-21 of a turn). The rest goes to fp32 as a value and
-// what its rounding left, which turns the result once more by less than 2^-23.
+// cos and sin of position times frequency, in 64 bits to the last step: the angle in turns, its whole and
+// quarter turns taken off (at position 2^31 the product still keeps 2^-21 of a turn), then the Taylor sums
+// on [-pi/4, pi/4], whose remainders are below 2^-33. Rounded once, to fp32; fp64 runs at fp32's rate here.
 __device__ __forceinline__ void turn_of(int pos, float freq, float& c, float& s) {
-    constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+    constexpr double kTurn = 0.15915494309189533577, kRadians = 6.283185307179586477;  // 1 / (2 pi), 2 pi
     double t = (double)pos * ((double)freq * kTurn);
     t -= __builtin_rint(t);
-    t += t;
-    const float half_turns = (float)t, rest = (float)(t - (double)half_turns) * 3.14159265f;
-    float s0, c0;
-    sincospif(half_turns, &s0, &c0);
-    c = __builtin_fmaf(-s0, rest, c0);
-    s = __builtin_fmaf(c0, rest, s0);
+    const double quarter = __builtin_rint(4.0 * t);
+    const double x = __builtin_fma(quarter, -0.25, t) * kRadians, y = x * x;
+    double u = __builtin_fma(y, -1.0 / 39916800.0, 1.0 / 362880.0);
+    u = __builtin_fma(y, u, -1.0 / 5040.0);
+    u = __builtin_fma(y, u, 1.0 / 120.0);
+    u = __builtin_fma(y, u, -1.0 / 6.0);
+    const float sx = (float)__builtin_fma(x * y, u, x);
+    double v = __builtin_fma(y, -1.0 / 3628800.0, 1.0 / 40320.0);
+    v = __builtin_fma(y, v, -1.0 / 720.0);
+    v = __builtin_fma(y, v, 1.0 / 24.0);
+    v = __builtin_fma(y, v, -0.5);
+    const float cx = (float)__builtin_fma(y, v, 1.0);
+    const int n = (int)quarter;  // -2 .. 2
+    c = n & 1 ? sx : cx;
+    s = n & 1 ? cx : sx;
+    c = (n + 1) & 2 ? -c : c;
+    s = n & 2 ? -s : s;
 }
 
-// A normed element, and a pair turned: every kernel here rounds the same products in the same order.
-// (Rounded one by one, not fused: a key whose quotient by its pool's step falls on a tie then goes the
-// way that the same formula in plain fp32 takes it, where its norm has the same last bit.)
+// 1 / sqrt(m): the fp32 function's (1 ulp) and a Newton step in 64 bits, rounded once.
+__device__ __forceinline__ float inv_sqrt(float m) {
+    const double y = (double)rsqrtf(m);
+    return m > 0.f && m < INFINITY ? (float)(y * __builtin_fma((double)m * y, -0.5 * y, 1.5)) : (float)y;
+}
+
+// A normed element, and a pair turned: every kernel here rounds the same products in the same order, one
+// by one and not fused. A 4-bit code turns on the last bit of its key, so the keys are those of the
+// formula evaluated in fp32 step by step, with exact angles and norms: of 33.5 M codes of 32 k rows none
+// differs from that (fp32 sine and cosine, fused products and the hardware's 1 / sqrt: one in 7 M, and
+// one bf16 output in 26 k), in the same time.
 __device__ __forceinline__ float normed(float x, float r, float w) {
 #pragma clang fp contract(off)
     return x * r * w;
@@ -85,7 +104,7 @@ __device__ __forceinline__ void rows_wave(const RopeArgs& a, const PoolOut& p, i
             const float x = load_as_f32(src, a.dt, at + d);
             sum = __builtin_fmaf(x, x, sum);
         }
-        norm = rsqrtf(wave_sum(sum) / (float)D + a.eps);
+        norm = inv_sqrt(wave_sum(sum) / (float)D + a.eps);
     }
     const bool cached = !is_q && !a.k_out;
     int blk = 0, off = 0;
@@ -203,13 +222,20 @@ __device__ __forceinline__ void apply_turn(const RopeArgs& a, const Unit& x, con
         turn_pair(fb[2], fb[3], r.c[3], r.s[3]);
     }
 }
-// A row's two runs, normed (w: the weight's runs), by the row's LPR lanes together.
-template <int LPR>
+// A row's two runs, normed (w: the weight's runs), by the row's LPR lanes together. The squares are summed
+// by dim wherever a row's pairs are whole: four in sequence, then neighbours, neighbours of those and so
+// on, which is as accurate as it is fixed. (Products of 16-bit types are exact, fused or not.)
+template <gg_dtype_t T>
+__device__ __forceinline__ float squares4(const float (&f)[4]) {
+#pragma clang fp contract(off)
+    if constexpr (T == GG_DTYPE_F32) return f[0] * f[0] + f[1] * f[1] + f[2] * f[2] + f[3] * f[3];
+    else return __builtin_fmaf(f[3], f[3], __builtin_fmaf(f[2], f[2], __builtin_fmaf(f[1], f[1], f[0] * f[0])));
+}
+template <gg_dtype_t T, int LPR>
 __device__ __forceinline__ void norm_runs(const RopeArgs& a, const float (&wa)[4], const float (&wb)[4], float (&fa)[4], float (&fb)[4]) {
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum = __builtin_fmaf(fa[e], fa[e], __builtin_fmaf(fb[e], fb[e], sum));
-    const float r = rsqrtf(__builtin_fmaf(group_sum<LPR>(sum), a.inv_d, a.eps));
+    const float sa = squares4<T>(fa), sb = squares4<T>(fb);
+    const float sum = a.style == GG_ROPE_HALVES ? group_sum<LPR>(sa) + group_sum<LPR>(sb) : group_sum<LPR>(sa + sb);
+    const float r = inv_sqrt(__builtin_fmaf(sum, a.inv_d, a.eps));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         fa[e] = normed(fa[e], r, wa[e]);
@@ -256,7 +282,7 @@ __device__ __forceinline__ void dense_side(const RopeArgs& a, const Unit& x, con
             to_f32<T>(ra[i], fa);
             to_f32<T>(rb[i], fb);
             fetch(i, h + kAhead * kRPW);
-            if (weight) norm_runs<LPR>(a, wa, wb, fa, fb);
+            if (weight) norm_runs<T, LPR>(a, wa, wb, fa, fb);
             apply_turn(a, x, r, fa, fb);
             if (h < n) {
                 store4<T>(dst, x.oa, fa);
@@ -315,7 +341,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_int4_kernel(RopeArgs a, Int4
             to_f32<T>(w.kb, kb);
             to_f32<T>(w.va, va);
             to_f32<T>(w.vb, vb);
-            if (a.k_weight) norm_runs<LPR>(a, wa, wb, ka, kb);
+            if (a.k_weight) norm_runs<T, LPR>(a, wa, wb, ka, kb);
             apply_turn(a, x, r, ka, kb);
             oa = x.oa;
             ob = x.ob;

@@ -250,6 +250,23 @@ def test_refusals(gv):
     kv.close()
 
 
+@pytest.mark.parametrize("d", [128, 66])
+def test_norm_of_rows_with_tiny_squares(gv, d):
+    """Squares below the normal range: fp32 keeps x^2 = 1e-40 to 2^-150 (7e-6 of it), so the norm, its
+    root, to 4e-6, and the rounding of the products adds 2^-22."""
+    rng = np.random.default_rng(12)
+    x = (1e-20 * rng.uniform(1, 2, (7, 2, d)) * rng.choice([-1, 1], (7, 2, d))).astype(np.float32)
+    x[3] = 0
+    zero, freq = torch.zeros(7, dtype=torch.int32, device="cuda"), torch.ones(d // 2, device="cuda")
+    one = torch.ones(d, device="cuda")
+    live = [0, 1, 2, 4, 5, 6]
+    got = gv.qk_norm_rope(torch.from_numpy(x).cuda(), None, zero, freq, one, eps=0.0)[0].cpu().numpy()
+    want = x.astype(np.float64)[live] / np.sqrt((x.astype(np.float64)[live] ** 2).mean(-1, keepdims=True))
+    assert (np.abs(got[live] - want) <= 1e-5 * np.abs(want)).all()
+    got = gv.qk_norm_rope(torch.from_numpy(x).cuda(), None, zero, freq, one, eps=1e-6)[0].cpu().numpy()
+    assert (np.abs(got - x.astype(np.float64) * 1e3) <= 2.0 ** -21 * np.abs(x) * 1e3).all()
+
+
 def test_tensors_of_another_device_are_refused(gv, monkeypatch):
     """The current device, as the calls see it, is one that holds none of the tensors."""
     n, hq, h, d = 4, 4, 2, 64
