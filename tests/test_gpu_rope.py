@@ -136,6 +136,8 @@ APPEND = [
     (384, 8, 2, 128, 16, 64, 1, "halves", "any"), (64, 4, 2, 64, 16, 32, 1, "halves", "run"), (37, 4, 2, 64, 16, 32, 2, "pairs", "any"),
     (20, 2, 1, 256, 16, 128, 1, "halves", "run"), (33, 3, 3, 128, 16, 32, 1, "halves", "run"), (33, 0, 2, 128, 16, 64, 1, "pairs", "run"),
     (18, 4, 2, 80, 8, 40, 1, "halves", "any"), (9, 2, 1, 34, 7, 10, 1, "pairs", "any"), (50, 8, 4, 128, 16, 0, 1, "halves", "run5"),
+    (70, 2, 3, 64, 16, 32, 1, "halves", "run"), (50, 2, 2, 256, 16, 128, 1, "halves", "run"), (50, 2, 1, 80, 16, 40, 1, "halves", "run"),
+    (40, 1, 2, 24, 16, 8, 1, "pairs", "run"), (40, 1, 1, 160, 16, 64, 1, "halves", "run5"), (40, 2, 1, 8, 16, 4, 1, "halves", "run"),
 ]
 
 
