@@ -2,7 +2,8 @@
 // step that gg_kv_append and gg_qk_norm_rope_append share.
 //
 // LPR lanes hold a row, two runs of four dims each (16 rows of one head at LPR 16, of two heads at 8;
-// at 32 two rounds of eight rows). Sixteen rows that are one block in order meet in LDS, and the block's
+// at 32 two rounds of eight rows). FULL: head_dim is 8 * LPR; else it is a smaller one of whole eights,
+// and the lanes past it hold nothing. Sixteen rows that are one block in order meet in LDS, and the block's
 // K tile, V tile (a byte to a token) and words go out in 16-byte runs, whole lines; other rows go out
 // two bytes of K and single bytes of V at a time, each a partial line. Workgroups of one row group are
 // neighbours, so that whole source rows are read at a time.
@@ -14,7 +15,9 @@
 
 namespace gg {
 
-constexpr int int4_tile_head_group(int head_dim) { return head_dim == 64 ? 2 : 1; }  // heads of a workgroup
+constexpr int int4_tile_head_group(int head_dim) { return head_dim <= 64 ? 2 : 1; }  // heads of a workgroup
+// (head_dims of whole eights up to 256)
+constexpr bool int4_tile_dim(int head_dim) { return head_dim % 8 == 0 && head_dim <= 256; }
 // Groups of sixteen rows: one more than the rows fill, as the first block may be entered anywhere.
 inline unsigned int4_tile_groups(int n_rows) { return (unsigned)((n_rows + 15 + 15) / 16); }
 inline unsigned int4_tile_heads(int heads, int head_dim) {
@@ -37,7 +40,7 @@ template <int LPR>
 struct Int4Tile {
     static constexpr int kD = 8 * LPR;
     static constexpr int kHeads = LPR == 8 ? 2 : 1;
-    __align__(16) uint8_t kv[kHeads][2][kD / 2 * 16];  // K tile, V tile
+    __align__(16) uint8_t kv[kHeads][kD * 16];  // K tile, V tile (head_dim * 8 bytes each)
     __align__(16) uint32_t words[kHeads][16];
 };
 
@@ -56,15 +59,17 @@ struct Int4Raw {
 // key's runs of dims oa .. oa + 3 and ob .. ob + 3 and the value's of 4u .. and D/2 + 4u .. ; it is
 // called before the row's slot is known. make(raw, r, h, u, ka, kb, va, vb, oa, ob) gives the values to be
 // stored, called with every lane of a row or none.
-template <gg_dtype_t T, int LPR, class FETCH, class MAKE>
+template <gg_dtype_t T, int LPR, bool FULL, class FETCH, class MAKE>
 __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t* slots, int n_rows, int group, int hg,
                                                Int4Tile<LPR>& tile, FETCH fetch, MAKE make) {
-    constexpr int D = Int4Tile<LPR>::kD, kRows = 256 / LPR;
+    constexpr int kRows = 256 / LPR;
+    const int D = FULL ? Int4Tile<LPR>::kD : p.D;
     constexpr int kRounds = LPR == 32 ? 2 : 1;
     // A prompt's groups start where its blocks do (rows that are not a prompt's may be grouped anyhow).
     const int s0 = slots[0];
     const int r0 = group * 16 - (s0 < 0 ? 0 : s0 % p.bs % 16);
     const int u = threadIdx.x % LPR;
+    const bool live = FULL || 8 * u < D;
     Int4Raw<T> raw[kRounds];
     int slot_of[kRounds];
     const int lead = slots[min(max(r0, 0), n_rows - 1)];
@@ -73,7 +78,8 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
     for (int round = 0; round < kRounds; ++round) {
         const int i = round * kRows + threadIdx.x / LPR, r = r0 + (i & 15), h = hg * Int4Tile<LPR>::kHeads + (i >> 4);
         slot_of[round] = slots[min(max(r, 0), n_rows - 1)];
-        raw[round] = fetch(min(max(r, 0), n_rows - 1), min(h, p.Hkv - 1), u);
+        if constexpr (!FULL) raw[round] = Int4Raw<T>{};
+        if (live) raw[round] = fetch(min(max(r, 0), n_rows - 1), min(h, p.Hkv - 1), u);
     }
 #pragma unroll
     for (int round = 0; round < kRounds; ++round) {
@@ -113,11 +119,12 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
             uint32_t vb4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) vb4[e] = int4_code(va[e], vs) | (int4_code(vb[e], vs) << 4);
+            if (!live) continue;
             if (whole) {
-                *(uint16_t*)&tile.kv[hl][0][row * (D / 2) + oa / 2] = (uint16_t)k01;
-                *(uint16_t*)&tile.kv[hl][0][row * (D / 2) + ob / 2] = (uint16_t)k23;
+                *(uint16_t*)&tile.kv[hl][row * (D / 2) + oa / 2] = (uint16_t)k01;
+                *(uint16_t*)&tile.kv[hl][row * (D / 2) + ob / 2] = (uint16_t)k23;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) tile.kv[hl][1][(4 * u + e) * 16 + row] = (uint8_t)vb4[e];
+                for (int e = 0; e < 4; ++e) tile.kv[hl][8 * D + (4 * u + e) * 16 + row] = (uint8_t)vb4[e];
                 if (u == 0) tile.words[hl][row] = word;
             } else {
                 uint8_t* kt = p.kc + p.tile0(blk, h) + (size_t)off * (D / 2);
@@ -136,7 +143,7 @@ __device__ __forceinline__ void int4_tile_rows(const Int4View& p, const int32_t*
     for (int i = threadIdx.x; i < Int4Tile<LPR>::kHeads * (D + 4); i += 256) {
         const int hl = i / (D + 4), j = i % (D + 4), h = hg * Int4Tile<LPR>::kHeads + hl;
         if (h >= p.Hkv) break;
-        if (j < D) *(uint4*)(p.kc + p.tile0(lead / 16, h) + (size_t)j * 16) = *(const uint4*)(&tile.kv[hl][0][0] + j * 16);
+        if (j < D) *(uint4*)(p.kc + p.tile0(lead / 16, h) + (size_t)j * 16) = *(const uint4*)&tile.kv[hl][j * 16];
         else ((uint4*)(p.words + p.word(lead / 16, h, 0)))[j - D] = ((const uint4*)tile.words[hl])[j - D];
     }
 }

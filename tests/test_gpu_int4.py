@@ -89,7 +89,8 @@ def test_append_is_the_rule(gv, d, bs, h, n, src, kind):
     kv.close()
 
 
-@pytest.mark.parametrize("first,n,d", [(0, 64, 128), (0, 1000, 128), (5, 300, 128), (13, 19, 64), (0, 16, 128), (1, 15, 128), (0, 100, 256)])
+@pytest.mark.parametrize("first,n,d", [(0, 64, 128), (0, 1000, 128), (5, 300, 128), (13, 19, 64), (0, 16, 128), (1, 15, 128), (0, 100, 256),
+                                       (0, 100, 96), (5, 70, 80), (0, 40, 8), (3, 50, 200)])
 def test_append_prompt_runs(gv, first, n, d):
     """Consecutive slots of whole and partial blocks of a shuffled table; neighbours in the first
     and last block keep their bytes."""
@@ -128,7 +129,8 @@ def test_append_of_offset_views(gv, src):
 
 @pytest.mark.parametrize("pool,d,bs", [(DType.INT4, 128, 16), (DType.INT4, 64, 16), (DType.INT4, 34, 7), (DType.INT4, 256, 16),
                                        (DType.INT8, 128, 16), (DType.FP8_E4M3, 128, 16), (DType.BF16, 64, 16),
-                                       (DType.F16, 80, 8), (DType.F32, 128, 16)])
+                                       (DType.F16, 80, 8), (DType.F32, 128, 16), (DType.INT4, 96, 16), (DType.INT4, 80, 16),
+                                       (DType.INT4, 208, 16), (DType.INT4, 40, 16), (DType.INT4, 16, 8)])
 @pytest.mark.parametrize("dst", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n", [1, 50])
 def test_read_gives_the_pool_back(gv, pool, d, bs, dst, n):
