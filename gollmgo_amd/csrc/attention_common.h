@@ -214,6 +214,7 @@ constexpr int kLptMaxSeqs = 1024;
 //     at 8 / 12 / 16 chunks of 32 tokens, 16 bf16 sequences of 256-1024 keys took 21.7 / 24.3 /
 //     21.1 and four of 1000-3000 keys 28.4 / 24.5 / 25.3.
 constexpr int kLptPieceNum = 2, kLptPieceDen = 1;  // items >= slots
+static_assert(kLptPieceNum >= 2 * kLptPieceDen, "lpt_pieces counts on pieces of at least twice the mean slot load");
 constexpr int kLptTSpan = 31;
 __host__ __device__ constexpr int lpt_min_chunks(int tok) { return tok == 64 ? 12 : 16; }
 //     4-bit pools at 8 / 12 chunks of 64: one sequence of 3000 keys 16.1 / 16.8 µs a planned call, 16

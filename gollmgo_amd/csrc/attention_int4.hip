@@ -29,10 +29,13 @@
 // p = 2^-12 that way, and half a step of 2^-35 B below; a piece whose scales lie further apart is
 // computed row by row in fp32. Each query row has a power of two of its own (its largest |q| in
 // [2^7, 2^8)), so rows do not touch.
-// PREC (fp32 queries or outputs): queries and p s_v in two f16 parts each, 22 bits, and the zero points
-// are taken from the codes in the operands (f16, exact). Summed apart, codes and zero points leave a
-// rounding of 2^-20 of the row's range, which f16 probabilities hide and fp32 results would show;
-// subtracting is 64 + 16 * 4 instructions more a chunk.
+// PREC (fp32 queries or outputs): queries and p s_v in two f16 parts each, 22 bits, and the codes less
+// their zero points as normal f16 numbers in the operands (exact). Two roundings that f16 probabilities
+// hide would show in fp32 results: codes and zero points summed apart leave 2^-20 of the row's range, and
+// the matrix unit aligns a subnormal's products by the exponent it is stored with, up to ten bits above
+// them, so that the sums keep about 17 bits (2-norm errors against 64 bits, 24
+// and 12 rows over 230 and 20 keys: 1.7e-5 and 1.3e-5 with subnormals, 4.5e-7 and 2.3e-7 with these).
+// Subtracting is 64 + 16 * 4 instructions more a chunk.
 //
 // Bound: one read of a token's 2 * (D / 2) + 4 bytes serves all its kv head's rows. Planned calls, 8 kv
 // heads of 128, bf16, kernel time: 64 sequences of 1024-8192 keys, 24 rows a head (two row tiles),
@@ -54,16 +57,21 @@ constexpr float kI4Spread = 4096.f;       // ratio of value scales that f16 prob
 constexpr float kI4Slack = 5.f;
 constexpr float kI4Unit = 1024.f;         // p s_v in units of B / kI4Unit: at most 2^15
 constexpr uint32_t kLoNib = 0x000f000fu, kHiNib = 0x00f000f0u;
+template <bool PREC>
+constexpr int kCodeExp = PREC ? 0 : 24;   // a code stands in its operand as n 2^-kCodeExp
 
-// Eight codes of a K dword as an MFMA operand: (n0, n4), 16 (n1, n5), (n2, n6), 16 (n3, n7).
-__device__ __forceinline__ uint4 k_operand8(uint32_t w) {
+// Eight codes of a K dword as an MFMA operand: (n0, n4), 16 (n1, n5), (n2, n6), 16 (n3, n7), of each pair
+// `base` more.
+__device__ __forceinline__ uint4 k_operand8(uint32_t w, uint32_t base) {
     const uint32_t u = w >> 8;
-    return make_uint4(w & kLoNib, w & kHiNib, u & kLoNib, u & kHiNib);
+    return make_uint4((w & kLoNib) | base, (w & kHiNib) | base, (u & kLoNib) | base, (u & kHiNib) | base);
 }
 
 __device__ __forceinline__ uint32_t pk_sub_f16(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, a) - __builtin_bit_cast(f16x2, b));
 }
+// PREC: codes and zero points as 1024 + n (f16 holds whole numbers there), whose difference is exact.
+constexpr uint32_t kF16_1024 = 0x64006400u;
 // An operand's codes less their zero points: z for the first and third pair, 16 z for the others.
 __device__ __forceinline__ uint4 less_zero(uint4 v, uint32_t z0, uint32_t z1, uint32_t z2, uint32_t z3) {
     return make_uint4(pk_sub_f16(v.x, z0), pk_sub_f16(v.y, z1), pk_sub_f16(v.z, z2), pk_sub_f16(v.w, z3));
@@ -198,8 +206,8 @@ struct Int4Queries {
             if (ch == 0) {
                 const float top = f16_bits_to_f32(f32_to_f16_bits(-sum));
                 s.qz[r] = f16_pair(top, -sum - top);
-                // (The codes are in units of 2^-24. Positive and finite: a hidden score times it stays -inf.)
-                const float mul = ldexpf(a.scale * kLog2e, k + 24);
+                // (Positive and finite: a hidden score times it stays -inf.)
+                const float mul = ldexpf(a.scale * kLog2e, k + kCodeExp<PREC>);
                 s.qmul[r] = fminf(fmaxf(mul, 0x1p-126f), 3.0e38f);
             }
         }
@@ -370,8 +378,11 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
                 for (int rt = 0; rt < NT; ++rt) qop[p][rt] = s.q[p][rt][mm][qlane];
 #pragma unroll
             for (int t = 0; t < kNS; ++t) {
-                uint4 kop = k_operand8(kr[t][mm]);
-                if constexpr (PREC) kop = less_zero(kop, kz[t], kz[t] << 4, kz[t], kz[t] << 4);
+                uint4 kop = k_operand8(kr[t][mm], PREC ? kF16_1024 : 0u);
+                if constexpr (PREC) {
+                    const uint32_t z0 = kz[t] | kF16_1024, z1 = (kz[t] << 4) | kF16_1024;
+                    kop = less_zero(kop, z0, z1, z0, z1);
+                }
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt)
 #pragma unroll
@@ -467,11 +478,12 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
             for (int i = 0; i < kVT; ++i) {
                 const uint32_t x = vr[i][2 * half], y = vr[i][2 * half + 1], x8 = x >> 8, y8 = y >> 8;
-                uint4 lo = make_uint4(x & kLoNib, x8 & kLoNib, y & kLoNib, y8 & kLoNib);
-                uint4 hi = make_uint4(x & kHiNib, x8 & kHiNib, y & kHiNib, y8 & kHiNib);
+                constexpr uint32_t b = PREC ? kF16_1024 : 0u;
+                uint4 lo = make_uint4((x & kLoNib) | b, (x8 & kLoNib) | b, (y & kLoNib) | b, (y8 & kLoNib) | b);
+                uint4 hi = make_uint4((x & kHiNib) | b, (x8 & kHiNib) | b, (y & kHiNib) | b, (y8 & kHiNib) | b);
                 if constexpr (PREC) {
-                    lo = less_zero(lo, z.x, z.y, z.z, z.w);
-                    hi = less_zero(hi, z.x << 4, z.y << 4, z.z << 4, z.w << 4);
+                    lo = less_zero(lo, z.x | b, z.y | b, z.z | b, z.w | b);
+                    hi = less_zero(hi, (z.x << 4) | b, (z.y << 4) | b, (z.z << 4) | b, (z.w << 4) | b);
                 }
 #pragma unroll
                 for (int rt = 0; rt < NT; ++rt)
@@ -505,7 +517,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         int4_piece_by_rows<HD>(a, kv, d, rows, 16 * NT, &s.o[wave][0][0]);
         return;
     }
-    const float unit = bound * (0x1p24f / kI4Unit);  // codes in 2^-24
+    const float unit = bound * ((float)(1 << kCodeExp<PREC>) / kI4Unit);
     for (int rt = 0; rt < NT; ++rt) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

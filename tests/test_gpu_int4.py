@@ -295,6 +295,28 @@ def check_attention(gv, kv, tables, rng, ctx, rows, R, hq, qdt="bf16", odt="bf16
     return got
 
 
+@pytest.mark.parametrize("d,hq,h,R,ctx,wide", [
+    (128, 9, 3, 8, [230, 238, 200, 31], None), (128, 3, 1, 4, [20] * 21, None), (128, 8, 2, 5, [1500, 700], 100),
+    (128, 8, 1, 6, [1200, 90], 100), (64, 8, 2, 5, [300, 1700], 110), (64, 16, 2, 8, [900, 33], 80)])
+@pytest.mark.parametrize("qdt", ["f32", "bf16"])
+def test_attention_fp32_outputs_in_norm(gv, d, hq, h, R, ctx, wide, qdt):
+    """The 2-norm of the error against 64 bits, which the largest deviations above do not bound closely.
+    An exponent's argument lies below 2^5: half a step of 2^-20, evenly spread 2^-20 ln 2 / sqrt(3) =
+    3.8e-7 of a probability; queries and probabilities to 22 bits and fp32 sums of products add less. Four
+    times that."""
+    say(f"int4 attention in norm d={d} q={hq}/{h} R={R} {ctx} {qdt}")
+    rng = np.random.default_rng(d + sum(ctx))
+    kv, tables = filled(gv, rng, ctx, h, d, 16, max_blocks=wide)
+    q = rng.normal(0, 1.5, (len(ctx), R, hq, d)).astype(np.float32)
+    qd, qf = to_dev(q, qdt)
+    out = torch.zeros(q.shape, device="cuda")
+    kv.attention(0, qd, out, torch.from_numpy(np.asarray(ctx, np.int32)).cuda(), torch.from_numpy(tables).cuda(), 1 / math.sqrt(d))
+    K, V, _, v_span = ref.pool_values(kv, 0, spans=True)
+    want = ref.attention(qf.astype(np.float64), K, V, ctx, [R] * len(ctx), tables, 1 / math.sqrt(d), np.zeros(q.shape), v_span)[0]
+    assert np.linalg.norm(out.double().cpu().numpy() - want) <= 1.5e-6 * np.linalg.norm(want)
+    kv.close()
+
+
 @pytest.mark.parametrize("partition", [64, 128, 1024])
 def test_attention_partitions(gv, partition):
     rng = np.random.default_rng(1)
