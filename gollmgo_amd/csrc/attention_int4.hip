@@ -9,7 +9,11 @@
 //   score     = s_k (sum q n - z_k sum q): the products run over the codes alone. The zero point is
 //               one more step of the contraction: operand (z, z) against (-sum q) in two f16 parts.
 //   P.V       = sum p s_v m - sum p s_v z_v: p s_v is the A operand, the codes and, as one more
-//               column tile, the zero points are B operands; the difference is taken at the end.
+//               column tile, the zero points are B operands; the difference is taken at the end. Both sums
+//               grow with the keys where their difference averages out, so each half of the dims has zero
+//               points in the units of its codes (columns 0..7: z, 8..15: 16 z): what the matrix unit cuts
+//               off the products is then alike in both and leaves with the difference (f16 outputs over 200 000 keys:
+//               8.0e-4 off in norm with one column for both halves, 2.4e-4 so, their own rounding 2.1e-4).
 // Codes go into the f16 operands without a conversion: the bits 0..15 (or 16 times that, the upper
 // half of a byte left in place) are the f16 subnormals n * 2^-24 (n * 2^-20), which
 // v_mfma_f32_16x16x32_f16 takes exactly. Eight codes cost one shift and four ands (an or with 0x6400
@@ -89,7 +93,7 @@ struct Int4Shared {
     // The chunk's tokens, decoded by the lane that loaded each token's word.
     float ks[kWaves][kTok], vs[kWaves][kTok];
     uint32_t kz[kWaves][kTok];                       // (z, z)
-    __align__(16) uint16_t vz[kWaves][kTok];         // in the order of the V operands
+    __align__(16) uint16_t vz[kWaves][kParts == 1 ? 2 : 1][kTok];  // in the order of the V operands: z, 16 z
     float m[kWaves][NT * 16], l[kWaves][NT * 16];
     int bad[kWaves];
     __align__(16) float o[kWaves][16][HD + 4];
@@ -349,7 +353,8 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
             s.ks[wave][own] = int4_k_scale(wr);
             s.vs[wave][own] = vs * vnorm;
             s.kz[wave][own] = zk | (zk << 16);
-            s.vz[wave][vz_at] = (uint16_t)int4_v_zero(wr);
+            s.vz[wave][0][vz_at] = (uint16_t)int4_v_zero(wr);
+            if constexpr (!PREC) s.vz[wave][1][vz_at] = (uint16_t)(int4_v_zero(wr) << 4);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -462,7 +467,7 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
         // ---- O += P . V, the zero points as one more column tile ----
 #pragma unroll
         for (int half = 0; half < kNS / 2; ++half) {
-            const uint4 z = *(const uint4*)&s.vz[wave][run + 8 * half];
+            const uint4 z = *(const uint4*)&s.vz[wave][PREC ? 0 : c16 >> 3][run + 8 * half];
             uint4 pa[NT][kParts];
 #pragma unroll
             for (int rt = 0; rt < NT; ++rt)
@@ -527,10 +532,12 @@ __device__ __forceinline__ void int4_piece(const AttnArgs& a, const KVView& kv, 
 #pragma unroll
             for (int u = 1; u < kWaves; ++u) mx = fmaxf(mx, s.m[u][r]);
             const float f = __builtin_amdgcn_exp2f(s.m[wave][r] - mx) * unit;
+            const float oz_other = dpp<0x128>(oz[rt][i]);  // row_ror:8
+            const float oz0 = c16 < 8 ? oz[rt][i] : oz_other, oz1 = c16 < 8 ? oz_other : oz[rt][i];
 #pragma unroll
             for (int t = 0; t < kVT; ++t) {
-                s.o[wave][rr][t * 16 + c16] = (o[rt][t][i] - oz[rt][i]) * f;
-                s.o[wave][rr][HD / 2 + t * 16 + c16] = (__builtin_fmaf(o[rt][t + kVT][i], 0.0625f, -oz[rt][i])) * f;
+                s.o[wave][rr][t * 16 + c16] = (o[rt][t][i] - oz0) * f;
+                s.o[wave][rr][HD / 2 + t * 16 + c16] = (o[rt][t + kVT][i] - oz1) * (0.0625f * f);
             }
         }
         __syncthreads();

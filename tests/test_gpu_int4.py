@@ -317,6 +317,26 @@ def test_attention_fp32_outputs_in_norm(gv, d, hq, h, R, ctx, wide, qdt):
     kv.close()
 
 
+@pytest.mark.parametrize("d,hq,h,R,ctx", [(128, 4, 1, 4, 60000), (64, 4, 2, 9, 24041), (128, 6, 1, 6, 30000), (128, 2, 2, 1, 40000)])
+@pytest.mark.parametrize("io", ["f16", "bf16"])
+def test_attention_long_contexts_in_norm(gv, d, hq, h, R, ctx, io):
+    """Over many keys the sums of codes and of zero points grow and their difference averages out. The
+    2-norm of the error against 64 bits: the output's rounding, and that of f16 probabilities, which for
+    values of either sign weighs as much as rounding f16 outputs: sqrt(2) of the f16 output's, less of the
+    bf16 one's. Half more than the output's own."""
+    say(f"int4 attention long d={d} q={hq}/{h} R={R} {ctx} {io}")
+    rng = np.random.default_rng(d + ctx)
+    kv, tables = filled(gv, rng, [ctx], h, d, 16)
+    qd, qf = to_dev(rng.normal(0, 1.5, (1, R, hq, d)).astype(np.float32), io)
+    out = torch.zeros(qd.shape, dtype=TORCH[io], device="cuda")
+    kv.attention(0, qd, out, torch.tensor([ctx], dtype=torch.int32, device="cuda"), torch.from_numpy(tables).cuda(), 1 / math.sqrt(d))
+    K, V, _, v_span = ref.pool_values(kv, 0, spans=True)
+    want = ref.attention(qf.astype(np.float64), K, V, [ctx], [R], tables, 1 / math.sqrt(d), np.zeros(qd.shape), v_span)[0]
+    least = np.linalg.norm(torch.from_numpy(want).to(TORCH[io]).double().numpy() - want)
+    assert np.linalg.norm(out.double().cpu().numpy() - want) <= 1.5 * least
+    kv.close()
+
+
 @pytest.mark.parametrize("partition", [64, 128, 1024])
 def test_attention_partitions(gv, partition):
     rng = np.random.default_rng(1)
