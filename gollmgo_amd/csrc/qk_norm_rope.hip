@@ -5,8 +5,8 @@
 // memory and a step's few rows by the launch. The angle is the dear part (40 instructions in 64 bits a
 // pair) and belongs to a row, not to a head: lanes hold the same pairs for every head they go through
 // and form their angles once. bf16, heads of 128, kernel time: 32768 rows of 32 + 8 heads, three position
-// axes, 671 MB 126.5 µs, 5.3 TB/s; 8192 rows with keys and values into a 4-bit pool, 177 MB 36.9 µs,
-// 4.8 TB/s; five rows 3.8 µs. Where pairs are not whole fours or rows are unaligned, a wave to a row and
+// axes, 671 MB 126.5 µs, 5.3 TB/s; 8192 rows with keys and values into a 4-bit pool, 177 MB 36.1 µs,
+// 4.9 TB/s; five rows 3.7 µs. Where pairs are not whole fours or rows are unaligned, a wave to a row and
 // head forms its own angles: 8192 rows of 40 heads 240 µs against 29.
 #include "gg_common.h"
 #include "int4.h"
